@@ -20,9 +20,12 @@ import numpy as np
 PKG_DIR = Path(__file__).resolve().parent.parent
 LIB_PATH = PKG_DIR / "libcoreg_b200.so"
 
-ACT_NONE, ACT_GELU, ACT_RELU, ACT_LEAKY, ACT_GELU_TANH = range(5)
+ACT_NONE, ACT_GELU, ACT_RELU, ACT_LEAKY, ACT_GELU_TANH, ACT_SILU = range(6)
 OPS_FP32, OPS_BF16 = 0, 1
 ERRORS_FATAL, ERRORS_RECORD = 0, 1
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_NTK, ROTARY_PARTS = range(4)
+ROTARY_MAX = 256
+I8_MAX_K = 131071
 
 
 class OclBackend(C.Structure):
@@ -67,6 +70,16 @@ class Opnd(C.Structure):
 
 class ConvGeom(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("kh", "kw", "sy", "sx", "py", "px", "dy", "dx", "groups")]
+
+
+class Rotary(C.Structure):
+    _fields_ = [
+        ("rot", C.c_int),
+        ("axes", C.c_int),
+        ("interleaved", C.c_int),
+        ("mscale", C.c_float),
+        ("step", C.c_uint64 * (ROTARY_MAX // 2)),
+    ]
 
 
 P = C.c_void_p
@@ -134,6 +147,15 @@ SIGNATURES = {
     "roma_local_corr_cl": (None, [C.POINTER(Ops), P, P, I, I, I, I, P, P]),
     "ops_gemm_noalloc": (None, [C.POINTER(Ops), I, I, I, Opnd, Opnd, I, Opnd, I, I, P, I, P, L, F, I, F]),
     "ops_gemm_noalloc_max_bytes": (C.c_size_t, []),
+    "ops_i8_ld": (I, [I]),
+    "ops_quant_i8": (None, [C.POINTER(Ops), L, I, Opnd, I, Opnd, P, L]),
+    "ops_gemm_i8": (None, [C.POINTER(Ops), I, I, I, Opnd, P, Opnd, P, P, Opnd, I, P, L, I, F]),
+    "ops_linear_i8_bytes": (SZ, [I, I]),
+    "ops_linear_i8": (None, [C.POINTER(Ops), I, I, I, Opnd, I, Opnd, P, P, Opnd, I, P, L, I, F, P]),
+    "ops_rotary_plan": (None, [C.POINTER(Rotary), I, I, I, C.c_double, I, C.c_double, L]),
+    "ops_rotary": (None, [C.POINTER(Ops), C.POINTER(Rotary), L, I, I, Opnd, Opnd, I, P, L]),
+    "ops_groupnorm_cl_bytes": (SZ, [I, L, I, I]),
+    "ops_groupnorm_cl": (None, [C.POINTER(Ops), I, L, I, I, Opnd, I, Opnd, I, P, P, F, I, F, P]),
     "ops_attention_qkv": (None, [C.POINTER(Ops), P, I, I, I, F, P]),
     "roma_gp_solve": (I, [C.POINTER(Ops), P, I, P, I, C.c_double, P]),
 }

@@ -94,6 +94,125 @@ void ops_gemm_noalloc(struct ops *o, int M, int N, int K, struct opnd A,
 /* Size in bytes of ops_gemm_noalloc's scratch array. */
 size_t ops_gemm_noalloc_max_bytes(void);
 
+/* ---- 8-bit linear layers, rotary positions, group norm ----
+ *
+ * Element types are named per buffer, apart from o->precision: OPS_FP32
+ * float, OPS_BF16 bfloat16 (offsets, leading dimensions and strides in
+ * elements of that type). The entry points below check their operands
+ * against the buffers' sizes, run on the ops context's device whichever
+ * the calling thread's current one is, allocate nothing, and may be
+ * captured into a CUDA graph; an empty call (no rows, no columns, no
+ * pixels) does nothing. Outputs may not overlap inputs but where said. */
+
+/* x sigmoid(x): an activation of the operations below only. */
+#define ACT_SILU 5
+
+/* Largest product depth of ops_gemm_i8: 2^17 - 1, so that no sum of
+ * products of 8-bit integers passes 32 bits. */
+#define OPS_I8_MAX_K 131071
+
+/* Row pitch in bytes of K 8-bit integers for ops_gemm_i8: K rounded up to
+ * a multiple of 16. */
+int ops_i8_ld(int K);
+
+/* Rows of X (rows x C, type xtype) to 8-bit integers with one scale each:
+ *   s = max |x| / 127 (float32, rounded to nearest), q = x / s
+ * rounded to the nearest integer (ties to even; decided on the exact
+ * quotient) within -127..127. Q holds bytes (Q.ld in bytes), S float32
+ * from element soff on, one per row. A row of zeros gets s = 0 and q = 0;
+ * a row that holds an infinity or NaN gets s = NaN and q = 0, so that the
+ * products of that row alone are NaN. Used for tokens (a scale per token)
+ * and for weights (W is out x in: a scale per output channel). No
+ * reference counterpart. */
+void ops_quant_i8(struct ops *o, long rows, int C, struct opnd X, int xtype, struct opnd Q,
+                  cl_mem S, long soff);
+
+/* C = act((A B^T) sa sb + bias) + R for 8-bit A (M x K, a scale sa[i] per
+ * row) and B (N x K, the PyTorch Linear layout, a scale sb[j] per row):
+ * the sums are exact 32-bit integers. A and B start at a multiple of 16
+ * bytes and their ld is one too (ops_i8_ld; bytes beyond K are not used).
+ * bias is float32 per column or NULL; R is NULL or a buffer of C's type
+ * and layout from element roff on, and may be C itself. ctype is the type
+ * of C and R. K is at most OPS_I8_MAX_K; K = 0 gives act(bias) + R. Few
+ * rows (up to 32) run a kernel that streams B once at memory speed, more
+ * the tcgen05 integer tensor cores. No reference counterpart (ops_gemm
+ * there is float32 only). */
+void ops_gemm_i8(struct ops *o, int M, int N, int K, struct opnd A, cl_mem sa, struct opnd B,
+                 cl_mem sb, cl_mem bias, struct opnd C, int ctype, cl_mem R, long roff, int act,
+                 float slope);
+
+/* Size in bytes of the work buffer of ops_linear_i8 (0: none needed). */
+size_t ops_linear_i8_bytes(int rows, int in);
+
+/* ops_linear over 8-bit weights: Y[rows, out] = act(X[rows, in] W^T + b)
+ * + R with X (type xtype) quantised per row as by ops_quant_i8, W and sw
+ * the weights' rows and scales as ops_quant_i8 left them, and the other
+ * arguments as in ops_gemm_i8 (Y is C there). The same result as
+ * ops_quant_i8 followed by ops_gemm_i8; few rows take one launch. work:
+ * at least ops_linear_i8_bytes(rows, in) bytes of device memory at a
+ * multiple of 16 bytes, NULL where that is 0; calls that may overlap in
+ * time (streams, graphs) each need their own. No reference counterpart. */
+void ops_linear_i8(struct ops *o, int rows, int in, int out, struct opnd X, int xtype,
+                   struct opnd W, cl_mem sw, cl_mem bias, struct opnd Y, int ytype, cl_mem R,
+                   long roff, int act, float slope, cl_mem work);
+
+/* Frequencies of a rotary encoding (ops_rotary_plan fills it). */
+#define OPS_ROTARY_MAX 256 /* Largest number of rotated columns. */
+struct ops_rotary {
+    int rot;         /* Rotated columns of each head, from its first on. */
+    int axes;        /* Positions per token: 1, or 2 (row and column). */
+    int interleaved; /* Pairs (2f, 2f + 1), or (f, f + rot / 2) with 0. */
+    float mscale;    /* Factor on the rotated columns. */
+    uint64_t step[OPS_ROTARY_MAX / 2]; /* Turns per position, in 2^-64. */
+};
+
+/* Frequency scalings: for positions beyond those a model was trained on. */
+#define OPS_ROTARY_PLAIN 0
+#define OPS_ROTARY_LINEAR 1 /* Every frequency over factor. */
+#define OPS_ROTARY_NTK 2    /* base times factor^(n / (n - 2)). */
+#define OPS_ROTARY_PARTS 3  /* Few turns over length: over factor; many: kept. */
+
+/* The frequencies of rot columns (even; a multiple of 2 axes): with n =
+ * rot / axes columns per axis, w_i = base^(-2 i / n) radians per position
+ * for i < n / 2, first those of axis 0, then those of axis 1. scaling
+ * changes them by factor (> 0): LINEAR divides them; NTK raises the base
+ * (n > 2); PARTS (the "NTK-by-parts" rule of YaRN, Peng et al. 2023)
+ * takes g w + (1 - g) w / factor with g = clamp((r - 1) / 31, 0, 1) for r =
+ * length w / 2 pi turns over the trained length, and sets mscale to
+ * 0.1 ln(factor) + 1 (1 otherwise). Host only; no device is needed. */
+void ops_rotary_plan(struct ops_rotary *r, int rot, int axes, int interleaved, double base,
+                     int scaling, double factor, long length);
+
+/* Rotary positions of rows x nh heads of d columns (a token's heads beside
+ * each other: the queries, or queries and keys, of a qkv buffer): Y = X
+ * with each pair (a, b) of a head's first r->rot columns replaced by
+ * mscale (a cos t - b sin t, a sin t + b cos t), t = w_f p, and the other
+ * columns as they were. p is pos0 plus the token's entry of pos (int32,
+ * rows x axes, packed), or pos0 + row with pos NULL (one axis only).
+ * Angles are kept as 64-bit fractions of a turn, exact to 2^-33 turns at
+ * any 31-bit position. Y may be X (in place: only rotated columns are
+ * read and written) or memory of its own. ops_rope is the float32 form
+ * with a table. No reference counterpart. */
+void ops_rotary(struct ops *o, const struct ops_rotary *r, long rows, int nh, int d,
+                struct opnd X, struct opnd Y, int type, cl_mem pos, long pos0);
+
+/* Size in bytes of the work buffer of ops_groupnorm_cl (0: none needed). */
+size_t ops_groupnorm_cl_bytes(int nimg, long HW, int C, int groups);
+
+/* Group norm with an activation over nimg channels-last maps (HW pixels
+ * of C channels; image i from X.off + i X.s0 on, pixels X.ld apart):
+ * Y = act((x - mean) / sqrt(var + eps) g[c] + b[c]) with the mean and the
+ * biased variance of each image's C / groups neighbouring channels over
+ * all pixels, held in float32; g and b float32 (both or neither NULL).
+ * Y may be X (the same offset, strides and type). work: at least
+ * ops_groupnorm_cl_bytes() bytes of device memory at a multiple of 16
+ * bytes, NULL where that is 0; calls that may overlap in time each need
+ * their own. No reference counterpart (ops_chan_stats and
+ * ops_chan_affine normalise single channels of channel-major maps). */
+void ops_groupnorm_cl(struct ops *o, int nimg, long HW, int C, int groups, struct opnd X,
+                      int xtype, struct opnd Y, int ytype, cl_mem g, cl_mem b, float eps,
+                      int act, float slope, cl_mem work);
+
 /* Non-zero when a bounded wait of a tensor-core kernel ran out since the
  * last call (the kernel then stopped and its results are invalid); the
  * code is cleared. */

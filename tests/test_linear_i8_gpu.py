@@ -1,0 +1,252 @@
+# SPDX-License-Identifier: Unlicense
+"""ops_quant_i8, ops_gemm_i8 and ops_linear_i8 against their plain forms in
+64 bits (GPU). The quantised values and scales are whole numbers and single
+roundings: they have to be equal.
+
+Products: the integer sum is exact; its conversion, the two scales and the
+bias are at most 5 roundings of 2^-24 of the terms' magnitude; the
+activation (Lipschitz constant below 1.2, its own error below 4 steps of its
+argument's magnitude, and for SiLU's fast exponential |v| 2^-22 more at
+|v| <= 30 relative to the result, which is at most |v|) stays within 32 such
+steps of the magnitude; the residual adds one of the sum, and the store half
+a step of the type."""
+
+import numpy as np
+import pytest
+
+import coreg
+from oracle import ops_b200_ref as ref
+from typed_ops import BF16, F32, HALF_STEP, Rows, close, rounded
+
+TYPES = {"f32": F32, "bf16": BF16}
+
+
+def tokens(rng, rows, C, t):
+    x = rng.standard_normal((rows, C)) * np.exp(rng.standard_normal((rows, 1)))
+    x[:, rng.random(C) < 0.02] *= 20
+    return rounded(x, t)
+
+
+def quant(dev, X, t, rows, C, qoff=0, qld=None):
+    Q = Rows(dev, rows, C, None, off=qoff, ld=C if qld is None else qld)
+    S = Rows(dev, rows, 1, F32, off=3)
+    dev.lib.ops_quant_i8(dev.ops_p, rows, C, X.opnd, t, Q.opnd, S.handle, 3)
+    return Q.read(), S.read()[:, 0]
+
+
+QUANT = [
+    # rows, C, X offset, X pitch, Q offset, Q pitch
+    (1, 1, 0, 1, 0, 1),
+    (3, 16, 0, 16, 0, 16),
+    (5, 17, 1, 19, 3, 21),
+    (2, 127, 0, 128, 0, 128),
+    (33, 256, 8, 264, 16, 272),
+    (9, 1024, 0, 1024, 0, 1024),
+    (7, 1000, 4, 1004, 0, 1008),
+    (4, 4096, 0, 4096, 0, 4096),
+    (3, 5000, 0, 5008, 0, 5008),
+    (2, 8192, 0, 8192, 0, 8192),
+    (2, 20001, 0, 20001, 5, 20003),
+    (1601, 96, 0, 96, 0, 96),
+    (1, 40000, 0, 40000, 0, 40000),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("shape", QUANT, ids=str)
+def test_quant_equals(dev, shape, t):
+    rows, C, xo, xl, qo, ql = shape
+    rng = np.random.default_rng(rows * 7 + C)
+    x = tokens(rng, rows, C, TYPES[t])
+    X = Rows(dev, rows, C, TYPES[t], x, off=xo, ld=xl)
+    q, s = quant(dev, X, TYPES[t], rows, C, qo, ql)
+    wq, ws = ref.quant_i8(x)
+    assert (s == ws).all()
+    assert (q == wq).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("C", [5, 48, 1024, 9000])
+def test_quant_edge_rows(dev, C, t):
+    """Zeros, infinities, NaN, the type's extremes, denormal rows and exact
+    ties (multiples of half a scale)."""
+    T = TYPES[t]
+    rng = np.random.default_rng(C)
+    big = np.float32(3.3e38)
+    x = np.zeros((14, C), np.float32)
+    x[1] = -0.0
+    x[2, C // 2] = np.inf
+    x[3] = rng.standard_normal(C)
+    x[3, C - 1] = np.nan
+    x[4] = rng.standard_normal(C)
+    x[4, 0] = -np.inf
+    x[5] = big * rng.uniform(-1, 1, C)
+    x[5, 1] = -big
+    x[6] = 1e-45 * rng.integers(-200, 201, C)
+    x[7] = 1e-40 * rng.standard_normal(C)
+    x[8] = 1e-37 * rng.standard_normal(C)
+    x[9] = 127.0
+    x[10] = rng.integers(-127, 127, C) + 0.5  # ties: the scale below is exactly 1
+    x[10, 0] = 127.0
+    x[11] = (rng.integers(-31, 31, C) + 0.5) * 2.0 ** -60
+    x[11, 0] = 127 * 2.0 ** -60
+    x[12, C - 1] = 1e-45
+    x[13] = 2.0 ** -91 * rng.standard_normal(C)
+    x = rounded(x, T)
+    q, s = quant(dev, Rows(dev, 14, C, T, x), T, 14, C)
+    wq, ws = ref.quant_i8(x)
+    np.testing.assert_array_equal(s, ws)
+    np.testing.assert_array_equal(q, wq)
+
+
+def i8_rows(dev, q, off=0, extra=0):
+    K = q.shape[1]
+    return Rows(dev, q.shape[0], K, None, q, off=off, ld=(K + 15) // 16 * 16 + extra)
+
+
+def operands(rng, M, N, K):
+    a = rng.integers(-127, 128, (M, K)).astype(np.int8)
+    b = rng.integers(-128, 128, (N, K)).astype(np.int8)
+    sa = np.exp(rng.standard_normal(M) - 4).astype(np.float32)
+    sb = np.exp(rng.standard_normal(N) - 5).astype(np.float32)
+    return a, sa, b, sb, rng.standard_normal(N).astype(np.float32)
+
+
+def tolerance(want, mag, res, t):
+    tol = 32 * 2.0 ** -24 * mag + HALF_STEP[t] * np.abs(want) + 1e-37
+    return tol + (2.0 ** -24 * (np.abs(want) + np.abs(res)) if res is not None else 0)
+
+
+GEMM = [
+    # M, N, K, extra pitch of A and B, C offset, C pitch beyond N
+    (1, 1, 1, 0, 0, 0),
+    (1, 1000, 1024, 0, 0, 0),
+    (2, 17, 40, 16, 1, 3),
+    (7, 64, 129, 0, 0, 0),
+    (8, 333, 2000, 0, 0, 0),
+    (9, 128, 64, 0, 8, 8),
+    (16, 96, 4096, 0, 0, 0),
+    (17, 100, 300, 0, 0, 0),
+    (31, 2049, 77, 0, 0, 1),
+    (32, 64, 512, 0, 0, 0),
+    (33, 65, 513, 16, 0, 0),
+    (64, 256, 1024, 0, 0, 0),
+    (100, 31, 100, 0, 0, 0),
+    (127, 129, 127, 0, 0, 0),
+    (128, 128, 128, 0, 0, 0),
+    (129, 257, 131, 32, 4, 4),
+    (200, 1000, 1111, 0, 0, 0),
+    (256, 256, 4096, 0, 0, 0),
+    (257, 513, 640, 0, 0, 0),
+    (700, 24, 48, 0, 0, 0),
+    (1000, 777, 333, 0, 0, 7),
+    (513, 16, 9000, 0, 0, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("shape", GEMM, ids=str)
+def test_gemm(dev, shape, t):
+    M, N, K, extra, co, cp = shape
+    T = TYPES[t]
+    rng = np.random.default_rng(M * 31 + N * 7 + K)
+    a, sa, b, sb, bias = operands(rng, M, N, K)
+    A, B = i8_rows(dev, a, 16, extra), i8_rows(dev, b, 0, extra)
+    SA, SB, BI = dev.upload(sa), dev.upload(sb), dev.upload(bias)
+    C = Rows(dev, M, N, T, off=co, ld=N + cp)
+    dev.lib.ops_gemm_i8(dev.ops_p, M, N, K, A.opnd, SA.handle, B.opnd, SB.handle, BI.handle,
+                        C.opnd, T, None, 0, 0, 0.1)
+    want, mag = ref.gemm_i8(a, sa, b, sb, bias)
+    close(C.read(), want, tolerance(want, mag, None, T))
+    assert dev.lib.coreg_tc_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("kind", ref.ACTS)
+@pytest.mark.parametrize("M", [5, 300])
+def test_gemm_activations_residual(dev, M, kind, t):
+    """Each activation, without a bias, with a residual of its own and in place."""
+    N, K, T = 200, 272, TYPES[t]
+    rng = np.random.default_rng(M + len(kind))
+    a, sa, b, sb, _ = operands(rng, M, N, K)
+    res = rounded(rng.standard_normal((M, N)), T)
+    A, B, SA, SB = i8_rows(dev, a), i8_rows(dev, b), dev.upload(sa), dev.upload(sb)
+    want, mag = ref.gemm_i8(a, sa, b, sb, None, kind, 0.1, res)
+    R, C = Rows(dev, M, N, T, res, off=8, ld=N + 8), Rows(dev, M, N, T, ld=N + 8)
+    D = Rows(dev, M, N, T, res, ld=N)
+    for out, r, roff in ((C, R.handle, 8), (D, D.handle, 0)):
+        dev.lib.ops_gemm_i8(dev.ops_p, M, N, K, A.opnd, SA.handle, B.opnd, SB.handle, None,
+                            out.opnd, T, r, roff, ref.ACTS.index(kind), 0.1)
+        close(out.read(), want, tolerance(want, mag, res, T))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 20, 140])
+def test_gemm_largest_sums(dev, M):
+    """The deepest product of the largest values: 2^31 - 2^14, exact; and K = 0."""
+    N, K = 40, coreg.I8_MAX_K
+    a = np.full((M, K), -128, np.int8)
+    b = np.full((N, K), -128, np.int8)
+    b[1::2] = 127
+    one = np.ones(max(M, N), np.float32)
+    A, B, S = i8_rows(dev, a), i8_rows(dev, b), dev.upload(one)
+    C = Rows(dev, M, N, F32)
+    dev.lib.ops_gemm_i8(dev.ops_p, M, N, K, A.opnd, S.handle, B.opnd, S.handle, None, C.opnd, F32,
+                        None, 0, 0, 0.0)
+    want = np.where(np.arange(N) % 2, -128.0 * 127 * K, 128.0 * 128 * K).astype(np.float32)
+    assert (C.read() == want).all()
+    bias = dev.upload(np.arange(N, dtype=np.float32) - 7)
+    dev.lib.ops_gemm_i8(dev.ops_p, M, N, 0, A.opnd, S.handle, B.opnd, S.handle, bias.handle,
+                        C.opnd, F32, None, 0, coreg.ACT_RELU, 0.0)
+    assert (C.read() == np.maximum(np.arange(N) - 7, 0)).all()
+
+
+LINEAR = [
+    # rows, in, out, X offset, X pitch beyond in
+    (1, 1, 3, 0, 0),
+    (1, 1024, 4096, 0, 0),
+    (2, 1000, 50, 0, 0),
+    (5, 37, 129, 3, 2),
+    (8, 4096, 256, 0, 0),
+    (16, 512, 512, 8, 8),
+    (17, 5000, 64, 0, 0),
+    (32, 2048, 100, 0, 0),
+    (33, 48, 48, 0, 0),
+    (130, 1024, 300, 0, 0),
+    (1601, 160, 96, 0, 16),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("xt", TYPES)
+@pytest.mark.parametrize("yt", TYPES)
+@pytest.mark.parametrize("shape", LINEAR, ids=str)
+def test_linear(dev, shape, xt, yt):
+    """Quantised exactly as by ops_quant_i8, so the product's bound holds for
+    the layer; a row with a NaN makes its own outputs NaN and no others."""
+    rows, K, N, xo, xp = shape
+    T = TYPES[yt]
+    rng = np.random.default_rng(rows + K + N)
+    x = tokens(rng, rows, K, TYPES[xt])
+    if rows > 4:
+        x[2] = 0
+        x[3, K // 3] = np.nan
+    w = rng.standard_normal((N, K)).astype(np.float32)
+    qw, sw = ref.quant_i8(w)
+    bias = rng.standard_normal(N).astype(np.float32)
+    res = rounded(rng.standard_normal((rows, N)), T)
+    X, W = Rows(dev, rows, K, TYPES[xt], x, off=xo, ld=K + xp), i8_rows(dev, qw)
+    SW, BI = dev.upload(sw), dev.upload(bias)
+    Y = Rows(dev, rows, N, T, res)
+    need = dev.lib.ops_linear_i8_bytes(rows, K)
+    work = dev.alloc(need) if need else None
+    dev.lib.ops_linear_i8(dev.ops_p, rows, K, N, X.opnd, TYPES[xt], W.opnd, SW.handle, BI.handle,
+                          Y.opnd, T, Y.handle, 0, coreg.ACT_GELU, 0.0, coreg.handle(work))
+    q, s = ref.quant_i8(x)
+    want, mag = ref.gemm_i8(q, s, qw, sw, bias, "gelu", 0, res)
+    close(Y.read(), want, tolerance(want, mag, res, T))
+    assert dev.lib.coreg_tc_status() == 0
