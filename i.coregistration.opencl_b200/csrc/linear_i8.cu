@@ -141,7 +141,7 @@ i8_tile_k(const I8Gemm g)
             if (r >= g.M || c >= g.N)
                 continue;
             float v = __int2float_rn(acc[i][j]) * g.sa[r] * g.sb[c] + (g.bias ? g.bias[c] : 0.0f);
-            v = g.act == ACT_SILU ? act_of<ACT_SILU>(v, 0.0f) : apply_act(v, g.act, g.slope);
+            v = act_any(v, g.act, g.slope);
             if (g.R)
                 v += ldf((const TC *)g.R + (long)r * g.ldc + c);
             stf((TC *)g.C + (long)r * g.ldc + c, v);

@@ -211,6 +211,15 @@ def test_groupnorm_refusals(h):
     h.refuses("overlaps", f, *args(y=M(X, 12, 4, 108)))
     h.refuses("overlaps", f, *args(y=M(X, 12, 0, 108), yt=BF16))
     h.refuses("overlaps", f, *args(g=Y, b=G))
+    need = h.lib.ops_groupnorm_cl_bytes(2, 9, 12, 3)
+    assert need > 0 and h.lib.ops_groupnorm_cl_bytes(0, 9, 12, 3) == 0
+    h.refuses("work buffer is NULL", f, *args())
+    h.refuses("work buffer .* passes", f, *args(work=h.buf(need - 1)))
+    h.refuses("work buffer is not 16-byte", f, *args(work=h.buf(BIG, 8)))
+    h.refuses("work buffer overlaps", f, *args(work=X))
+    h.refuses("work buffer overlaps", f, *args(work=Y))
+    h.refuses("maps of", f, *args(n=65536))
+    h.refuses("maps of", f, *args(hw=2 ** 30 + 1))
     h.runs_nothing(f, *args(n=0))
     h.runs_nothing(f, *args(hw=0))
     h.runs_nothing(f, *args(c=0, groups=1))
