@@ -5,7 +5,7 @@
 
 #include <type_traits>
 
-#include "opcheck.cuh"
+#include "linear_i8.cuh"
 
 using namespace coreg;
 
@@ -14,100 +14,226 @@ namespace {
 
 // ------------------------------------------------------------ quantisation
 
-// The nearest integer (ties to even) to the real quotient x / s, |x| <= 127 s
-// up to a rounding of s. r = x (1 / s) is off by less than 2^-15, so its
-// nearest integer q is off by at most one, and only next to a tie. x - q s is
+// A row's scale from the bits of its largest magnitude (an unsigned
+// comparison orders finite < infinite < NaN) and its quotients.
+//
+// The nearest integer (ties to even) to the real quotient x / s: r = x (1 / s)
+// rounded to an integer by adding and taking off 1.5 2^23 is off by at most
+// one, and only next to a tie (r itself is off by less than 2^-15). x - q s is
 // exact in one fused multiply-add: x and s are multiples of the smaller of
 // their last places, and the difference is below s (in units of that place
-// below 2^24). So |2 (x - q s)| against s decides, without a division.
-__device__ __forceinline__ int nearest_quotient(float x, float s, float inv)
-{
-    float q = rintf(x * inv);
-    const float d = fmaf(-q, s, x), e = fabsf(d + d);
-    if (e > s || (e == s && ((int)q & 1)))
-        q += copysignf(1.0f, d);
-    return (int)fminf(fmaxf(q, -127.0f), 127.0f);
-}
-
-// A row's scale from the bits of its largest magnitude (an unsigned
-// comparison orders finite < infinite < NaN), and what its quotients take:
-// scales below 2^-90, whose reciprocal could overflow, go with their values
-// into the normal range by an exact power of two.
+// below 2^24). So |x - q s| against s / 2 decides, without a division, and
+// the seldom value that it moves takes a branch.
 struct RowScale {
-    float s, up, s_up, inv;
+    float s, inv, half;
+    bool tiny; // s below 2^-90: 1 / s could overflow, s could be denormal
     __device__ explicit RowScale(uint32_t amax)
     {
         if (amax >= 0x7f800000u) {
             s = __int_as_float(0x7fffffff);
-            up = s_up = inv = 0.0f;
+            inv = half = 0.0f;
+            tiny = false;
             return;
         }
         s = __fdiv_rn(__uint_as_float(amax), 127.0f);
-        up = s < 0x1p-90f ? 0x1p+90f : 1.0f;
-        s_up = s * up;
-        inv = s > 0.0f ? __fdiv_rn(1.0f, s_up) : 0.0f;
+        tiny = s < 0x1p-90f;
+        inv = tiny ? 0.0f : __fdiv_rn(1.0f, s);
+        half = 0.5f * s;
     }
-    // The quantised value; 0 in rows without a positive finite scale.
-    __device__ int of(float x) const
+    // The quantised value as the low byte of the result.
+    __device__ __forceinline__ uint32_t of(float x) const
     {
-        return inv > 0.0f ? nearest_quotient(x * up, s_up, inv) : 0;
+        const float big = fmaf(x, inv, 12582912.0f), q = big - 12582912.0f;
+        const float d = fmaf(-q, s, x);
+        if (fabsf(d) < half)
+            return __float_as_uint(big);
+        return slow(x, q, d);
+    }
+    // Values next to a tie, and rows without a normal positive scale.
+    __device__ __noinline__ uint32_t slow(float x, float q, float d) const
+    {
+        if (tiny) {
+            // Into the normal range by an exact power of two.
+            const float up = s * 0x1p+90f;
+            if (!(up > 0.0f))
+                return 0;
+            x *= 0x1p+90f;
+            q = rintf(__fdiv_rn(x, up));
+            d = fmaf(-q, up, x);
+            const float e = fabsf(d + d);
+            if (e > up || (e == up && ((int)q & 1)))
+                q += copysignf(1.0f, d);
+        }
+        else if (!(s > 0.0f)) {
+            return 0; // a row with an infinity or NaN
+        }
+        else if (fabsf(d) > half || ((int)q & 1)) {
+            q += copysignf(1.0f, d);
+        }
+        return (uint32_t)(int)fminf(fmaxf(q, -127.0f), 127.0f);
     }
 };
 
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// One block per row, two passes over it.
+// Four quantised values in a word.
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// 16 bytes of a row: V values, or one value where rows are not aligned.
+template <typename T, int V>
+struct Piece {
+    uint4 w;
+    __device__ __forceinline__ void load(const T *p) { w = *(const uint4 *)p; }
+    __device__ __forceinline__ float at(int e) const
+    {
+        const int i = sizeof(T) == 4 ? e : e / 2;
+        const uint32_t x = i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
+        return __uint_as_float(sizeof(T) == 4 ? x : e % 2 ? x & 0xffff0000u : x << 16);
+    }
+    __device__ __forceinline__ uint32_t top() const
+    {
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < V; e++)
+            m = max(m, magnitude(at(e)));
+        return m;
+    }
+    __device__ __forceinline__ void store(int8_t *q, const RowScale &s) const
+    {
+        const uint32_t a = pack4(s.of(at(0)), s.of(at(1)), s.of(at(2)), s.of(at(3)));
+        if constexpr (V == 4)
+            *(uint32_t *)q = a;
+        else
+            *(uint2 *)q = make_uint2(a, pack4(s.of(at(4)), s.of(at(5)), s.of(at(6)), s.of(at(7))));
+    }
+};
+
 template <typename T>
+struct Piece<T, 1> {
+    float f;
+    __device__ __forceinline__ void load(const T *p) { f = ldf(p); }
+    __device__ __forceinline__ uint32_t top() const { return magnitude(f); }
+    __device__ __forceinline__ void store(int8_t *q, const RowScale &s) const
+    {
+        *q = (int8_t)s.of(f);
+    }
+};
+
+// G threads of a block of 256 per row, its pieces in their registers (NP a
+// thread) from the maximum to the result, so that a row is read once; longer
+// rows read what is beyond again. Values behind the last whole piece one by
+// one.
+template <typename T, int V, int G, int NP>
 __global__ void __launch_bounds__(256)
-quant_row_k(const T *X, long ldx, int C, int8_t *Q, long ldq, float *S)
+quant_k(const T *X, long ldx, long rows, int C, int8_t *Q, long ldq, float *S)
 {
     __shared__ uint32_t red[8];
-    const long row = blockIdx.x;
-    const T *x = X + row * ldx;
+    const int lane = threadIdx.x % G;
+    const long row = (long)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const bool here = row < rows;
+    const T *x = X + (here ? row : 0) * ldx;
+    const int n = here ? C / V : 0; // whole pieces
+    Piece<T, V> r[NP];
     uint32_t m = 0;
-    for (int c = threadIdx.x; c < C; c += blockDim.x)
-        m = max(m, magnitude(ldf(x + c)));
+#pragma unroll
+    for (int i = 0; i < NP; i++)
+        if (lane + i * G < n)
+            r[i].load(x + (long)(lane + i * G) * V);
+#pragma unroll
+    for (int i = 0; i < NP; i++)
+        if (lane + i * G < n)
+            m = max(m, r[i].top());
+    for (int k = lane + NP * G; k < n; k += G) {
+        Piece<T, V> f;
+        f.load(x + (long)k * V);
+        m = max(m, f.top());
+    }
+    const int c = n * V + lane; // its value behind the pieces (C % V < G)
+    const bool odd = here && c < C;
+    float f = 0.0f;
+    if (odd) {
+        f = ldf(x + c);
+        m = max(m, magnitude(f));
+    }
     m = __reduce_max_sync(0xffffffffu, m);
-    if (threadIdx.x % 32 == 0)
-        red[threadIdx.x / 32] = m;
-    __syncthreads();
-    for (int w = 0; w < 8; w++)
-        m = max(m, red[w]);
-    const RowScale rs(m);
-    if (threadIdx.x == 0)
-        S[row] = rs.s;
-    for (int c = threadIdx.x; c < C; c += blockDim.x)
-        Q[row * ldq + c] = (int8_t)rs.of(ldf(x + c));
+    if (G > 32) {
+        if (threadIdx.x % 32 == 0)
+            red[threadIdx.x / 32] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < G / 32; w++)
+            m = max(m, red[threadIdx.x / G * (G / 32) + w]);
+    }
+    if (!here)
+        return;
+    const RowScale s(m);
+    if (lane == 0)
+        S[row] = s.s;
+    int8_t *q = Q + row * ldq;
+#pragma unroll
+    for (int i = 0; i < NP; i++)
+        if (lane + i * G < n)
+            r[i].store(q + (long)(lane + i * G) * V, s);
+    for (int k = lane + NP * G; k < n; k += G) {
+        Piece<T, V> f2;
+        f2.load(x + (long)k * V);
+        f2.store(q + (long)k * V, s);
+    }
+    if (odd)
+        q[c] = (int8_t)s.of(f);
+}
+
+template <typename T, int V>
+void quant_launch(cudaStream_t st, const View &x, int8_t *q, long ldq, float *s)
+{
+    // A warp per row up to 8 pieces a lane, then a quarter of a block, then a
+    // block.
+    const int pieces = (int)(x.cols / V);
+    const T *p = (const T *)x.p;
+    auto go = [&](auto g, auto np) {
+        constexpr int G = decltype(g)::value, NP = decltype(np)::value;
+        quant_k<T, V, G, NP><<<cdiv(x.rows, 256 / G), 256, 0, st>>>(p, x.ld, x.rows, (int)x.cols, q,
+                                                                    ldq, s);
+    };
+    typedef std::integral_constant<int, 32> warp;
+    typedef std::integral_constant<int, 64> two;
+    typedef std::integral_constant<int, 256> block;
+    typedef std::integral_constant<int, 4> four;
+    typedef std::integral_constant<int, 8> eight;
+    if (pieces <= 32 * 4)
+        go(warp(), four());
+    else if (pieces <= 64 * 4)
+        go(two(), four());
+    else
+        go(block(), eight());
 }
 
 void quant_rows(cudaStream_t st, const View &x, int xtype, int8_t *q, long ldq, float *s)
 {
-    if (xtype == OPS_BF16)
-        quant_row_k<<<(unsigned)x.rows, 256, 0, st>>>((const __nv_bfloat16 *)x.p, x.ld,
-                                                      (int)x.cols, q, ldq, s);
+    const int V = xtype == OPS_BF16 ? 8 : 4;
+    const bool al = ((uintptr_t)x.p & 15) == 0 && (x.rows == 1 || x.ld % V == 0) &&
+                    (uintptr_t)q % V == 0 && (x.rows == 1 || ldq % V == 0);
+    if (xtype == OPS_BF16 && al)
+        quant_launch<__nv_bfloat16, 8>(st, x, q, ldq, s);
+    else if (xtype == OPS_BF16)
+        quant_launch<__nv_bfloat16, 1>(st, x, q, ldq, s);
+    else if (al)
+        quant_launch<float, 4>(st, x, q, ldq, s);
     else
-        quant_row_k<<<(unsigned)x.rows, 256, 0, st>>>((const float *)x.p, x.ld, (int)x.cols, q,
-                                                      ldq, s);
+        quant_launch<float, 1>(st, x, q, ldq, s);
 }
 
 // ----------------------------------------------------------------- product
 
-struct I8Gemm {
-    int M, N, K;
-    const int8_t *A;
-    long lda;
-    const float *sa;
-    const int8_t *B;
-    long ldb;
-    const float *sb;
-    const float *bias; // per column or NULL
-    void *C;
-    long ldc;
-    const void *R; // C's layout and type, or NULL
-    int c_bf16;
-    int act;
-    float slope;
-};
+// A sum as a value before the activation. (The token's scale first: the two
+// scales' own product could pass the type's range where the result does not.)
+__device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias)
+{
+    return fmaf(__int2float_rn(acc) * sa, sb, bias);
+}
 
 // 64 x 64 output tiles, 4 x 4 sums per thread, 64 bytes of depth staged at a
 // time; four products per __dp4a.
@@ -140,7 +266,7 @@ i8_tile_k(const I8Gemm g)
             const int r = m0 + ty + 16 * i, c = n0 + tx + 16 * j;
             if (r >= g.M || c >= g.N)
                 continue;
-            float v = __int2float_rn(acc[i][j]) * g.sa[r] * g.sb[c] + (g.bias ? g.bias[c] : 0.0f);
+            float v = scaled(acc[i][j], g.sa[r], g.sb[c], g.bias ? g.bias[c] : 0.0f);
             v = act_any(v, g.act, g.slope);
             if (g.R)
                 v += ldf((const TC *)g.R + (long)r * g.ldc + c);
@@ -148,8 +274,117 @@ i8_tile_k(const I8Gemm g)
         }
 }
 
-void gemm_i8(cudaStream_t st, const I8Gemm &g)
+// Few rows: the weights stream once from memory, so a block takes 16 of
+// their rows (output channels), its 8 warps the depth by turns of 64 bytes.
+// mma.m16n8k32 of 8-bit integers with the weights as the 16 rows and 8 tokens
+// as the columns: lane l's operands are four words of channel (or token) l /
+// 4, and as the order of the depth is free as long as both operands agree,
+// they are one 16-byte load at 16 (l % 4) of the turn. The warps' sums meet
+// in shared memory.
+constexpr int SK_CH = 16, SK_WARPS = 8, SK_TURN = 64;
+
+__device__ __forceinline__ void mma_s8(int d[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                       uint32_t a3, uint32_t b0, uint32_t b1)
 {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+                 "{%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16 bytes of a row from depth k on, zeros behind K: the bytes there need not
+// exist.
+__device__ __forceinline__ uint4 load16(const int8_t *row, int k, int K)
+{
+    if (k + 16 <= K)
+        return *(const uint4 *)(row + k);
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+        if (k + i < K)
+            w[i / 4] |= (uint32_t)(uint8_t)row[k + i] << (8 * (i % 4));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// NT: groups of 8 tokens.
+template <int NT, typename TC>
+__global__ void __launch_bounds__(32 * SK_WARPS)
+i8_skinny_k(const I8Gemm g)
+{
+    __shared__ int part[SK_WARPS][SK_CH][8 * NT + 1];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, n0 = blockIdx.x * SK_CH;
+    const int r = lane / 4, kk = 16 * (lane % 4);
+    const int8_t *w0 = g.B + (long)min(n0 + r, g.N - 1) * g.ldb;
+    const int8_t *w1 = g.B + (long)min(n0 + r + 8, g.N - 1) * g.ldb;
+    int d[NT][4] = {};
+    constexpr int U = NT == 4 ? 2 : 4, STEP = SK_WARPS * SK_TURN;
+    for (int k0 = warp * SK_TURN + kk; k0 < g.K + kk; k0 += U * STEP) {
+        uint4 a[U], b[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            a[u] = load16(w0, k0 + u * STEP, g.K);
+            b[u] = load16(w1, k0 + u * STEP, g.K);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const int m = 8 * t + r;
+                const uint4 x = m < g.M ? load16(g.A + (long)m * g.lda, k0 + u * STEP, g.K)
+                                        : make_uint4(0, 0, 0, 0);
+                mma_s8(d[t], a[u].x, b[u].x, a[u].y, b[u].y, x.x, x.y);
+                mma_s8(d[t], a[u].z, b[u].z, a[u].w, b[u].w, x.z, x.w);
+            }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            part[warp][r + 8 * (i / 2)][8 * t + 2 * (lane % 4) + i % 2] = d[t][i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < SK_CH * g.M; e += 32 * SK_WARPS) {
+        const int c = e % SK_CH, m = e / SK_CH;
+        if (n0 + c >= g.N)
+            continue;
+        int acc = 0;
+#pragma unroll
+        for (int w = 0; w < SK_WARPS; w++)
+            acc += part[w][c][m];
+        float v = scaled(acc, g.sa[m], g.sb[n0 + c], g.bias ? g.bias[n0 + c] : 0.0f);
+        v = act_any(v, g.act, g.slope);
+        const long at = (long)m * g.ldc + n0 + c;
+        if (g.R)
+            v += ldf((const TC *)g.R + at);
+        stf((TC *)g.C + at, v);
+    }
+}
+
+template <typename TC>
+void skinny(cudaStream_t st, const I8Gemm &g)
+{
+    const unsigned grid = cdiv(g.N, SK_CH);
+    if (g.M <= 8)
+        i8_skinny_k<1, TC><<<grid, 32 * SK_WARPS, 0, st>>>(g);
+    else if (g.M <= 16)
+        i8_skinny_k<2, TC><<<grid, 32 * SK_WARPS, 0, st>>>(g);
+    else
+        i8_skinny_k<4, TC><<<grid, 32 * SK_WARPS, 0, st>>>(g);
+}
+
+constexpr int SKINNY_ROWS = 32;
+
+void gemm_i8(const struct ocl_backend *ocl, const I8Gemm &g)
+{
+    cudaStream_t st = stream_of(ocl);
+    if (g.M <= SKINNY_ROWS) {
+        if (g.c_bf16)
+            skinny<__nv_bfloat16>(st, g);
+        else
+            skinny<float>(st, g);
+        return;
+    }
+    if (g.K > 0 && gemm_i8_tc(st, g, sms_of(ocl)))
+        return;
     const dim3 grid(cdiv(g.N, 64), cdiv(g.M, 64));
     if (g.c_bf16)
         i8_tile_k<__nv_bfloat16><<<grid, 256, 0, st>>>(g);
@@ -288,7 +523,7 @@ extern "C" void ops_gemm_i8(struct ops *o, int M, int N, int K, struct opnd A, c
     if (!dev.ok)
         return;
     Prof p(o->ocl, "gemm_i8");
-    gemm_i8(stream_of(o->ocl), g);
+    gemm_i8(o->ocl, g);
     launch_ok("gemm_i8");
 }
 
@@ -338,6 +573,6 @@ extern "C" void ops_linear_i8(struct ops *o, int rows, int in, int out, struct o
     g.A = q;
     g.lda = ops_i8_ld(in);
     g.sa = (const float *)ws.p;
-    gemm_i8(st, g);
+    gemm_i8(o->ocl, g);
     launch_ok("linear_i8");
 }

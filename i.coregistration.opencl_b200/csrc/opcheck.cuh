@@ -148,14 +148,22 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
 
 __device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
 
-// Exact GELU, x Phi(x) = (x + |x| erf(|x| / sqrt 2)) / 2, of two values. With a =
-// min(|x|, 5.4), erf(a / sqrt 2) = a P(a^2), P the polynomial of degree 14 in s =
-// 2 a^2 / 5.4^2 - 1 with the least largest error a |P - exact| (fitted here in
-// 64 bits; 6e-8), evaluated in float32: off by at most 2.4e-7, as 0.5 (1 +
-// erff) is by 1.2e-7. At 5.4 it reaches 1 (min), so that large |x| give
-// exactly x or 0. Written for the packed multiply-add: 12 issue slots a
-// value, about half of CUDA's erff in the same formula, which bounded the
-// epilogue of the 8-bit product.
+// a b + c clamped to 0..1 (0 for NaN).
+__device__ __forceinline__ float fma_sat(float a, float b, float c)
+{
+    float d;
+    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// Exact GELU, x Phi(x), of two values. Phi(x) = 0.5 + x Q(min(x^2, 5.4^2)),
+// clamped to 0..1, where Q is the polynomial of degree 14 in s = 2 x^2 / 5.4^2 -
+// 1 with the least largest error of x Q over |x| <= 5.4 (fitted here in 64
+// bits; 3e-8); evaluated in float32 Phi is off by at most 1.2e-7, as 0.5 (1 +
+// erff(x / sqrt 2)) is by 0.6e-7. At 5.4 x Q passes 0.5, so that larger |x|
+// give exactly x or 0. All but four operations of a pair are packed: 10.5
+// issue slots a value, half of CUDA's erff in the same formula, which
+// bounded the epilogue of the 8-bit product.
 __device__ __forceinline__ float2 gelu2(float2 x)
 {
     constexpr float P[15] = {
@@ -164,17 +172,22 @@ __device__ __forceinline__ float2 gelu2(float2 x)
         0.03929029032588005f,   -0.027926640585064888f, 0.01930239051580429f,
         -0.01343067642301321f,  0.007317845709621906f,  -0.002372820395976305f,
         0.0017498668748885393f, -0.0020567376632243395f, 0.0007857177406549454f};
-    const float2 ax = make_float2(fabsf(x.x), fabsf(x.y));
-    const float2 a = make_float2(fminf(ax.x, 5.4f), fminf(ax.y, 5.4f));
-    const float2 u = make_float2(a.x * a.x, a.y * a.y);
+    float2 u = fma2(x, x, pair(0.0f));
+    u = make_float2(fminf(u.x, 5.4f * 5.4f), fminf(u.y, 5.4f * 5.4f));
     const float2 s = fma2(u, pair(2.0f / (5.4f * 5.4f)), pair(-1.0f));
-    float2 p = pair(P[14]);
+    float2 q = pair(0.5f * P[14]);
 #pragma unroll
     for (int i = 13; i >= 0; i--)
-        p = fma2(p, s, pair(P[i]));
-    const float2 e = make_float2(fminf(a.x * p.x, 1.0f), fminf(a.y * p.y, 1.0f));
-    const float2 y = fma2(ax, e, x);
-    return make_float2(0.5f * y.x, 0.5f * y.y);
+        q = fma2(q, s, pair(0.5f * P[i]));
+    return fma2(x, make_float2(fma_sat(x.x, q.x, 0.5f), fma_sat(x.y, q.y, 0.5f)), pair(0.0f));
+}
+
+// The larger value, or NaN where one is (fmaxf would drop it).
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
 }
 
 // v / (1 + e^-t) by the fast exponential and division: relative error below
@@ -192,7 +205,7 @@ __device__ __forceinline__ float2 act2(float2 v, float slope)
     if (ACT == ACT_GELU)
         return gelu2(v);
     if (ACT == ACT_RELU)
-        return make_float2(fmaxf(v.x, 0.0f), fmaxf(v.y, 0.0f));
+        return make_float2(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f));
     if (ACT == ACT_LEAKY)
         return make_float2(v.x >= 0.0f ? v.x : slope * v.x, v.y >= 0.0f ? v.y : slope * v.y);
     if (ACT == ACT_GELU_TANH) {

@@ -715,6 +715,7 @@ int attn_status()
 
 int gemm_status();
 int dwpw_status();
+int i8_status();
 
 }  // namespace tc
 
@@ -741,5 +742,6 @@ extern "C" int coreg_tc_status(void)
     const int a = coreg::tc::gemm_status();
     const int b = coreg::tc::attn_status();
     const int c = coreg::tc::dwpw_status();
-    return a ? a : b ? b : c;
+    const int d = coreg::tc::i8_status();
+    return a ? a : b ? b : c ? c : d;
 }

@@ -338,6 +338,12 @@ bool make_map_conv(CUtensorMap *map, const void *base, int H, int W, int C, int 
 // (2-D) or TW x TH pixels (3-D), 128-byte swizzle.
 bool make_map_out(CUtensorMap *map, void *base, int es, long rows, long cols, long ld,
                   int conv, int H, int W, int TW, int TH);
+// Host: 2-D tensor map of a row-major matrix of bytes, bfloat16 or float (es 1,
+// 2 or 4; rows `pitch` bytes apart), boxes of box_cols x box_rows with
+// swizzle_bytes 128 or 64, zero fill outside; false unless the base and the
+// pitch are multiples of 16 bytes.
+bool make_map_rows(CUtensorMap *map, const void *base, int es, long rows, long cols, long pitch,
+                   int box_cols, int box_rows, int swizzle_bytes);
 // Host: opt in to `bytes` of dynamic shared memory for kernel `fn` on the
 // current device (once per device).
 bool smem_opt_in(const void *fn, size_t bytes, unsigned *done_mask);
