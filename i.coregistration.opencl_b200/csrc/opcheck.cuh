@@ -156,29 +156,39 @@ __device__ __forceinline__ float fma_sat(float a, float b, float c)
     return d;
 }
 
-// Exact GELU, x Phi(x), of two values. Phi(x) = 0.5 + x Q(min(x^2, 5.4^2)),
-// clamped to 0..1, where Q is the polynomial of degree 14 in s = 2 x^2 / 5.4^2 -
-// 1 with the least largest error of x Q over |x| <= 5.4 (fitted here in 64
-// bits; 3e-8); evaluated in float32 Phi is off by at most 1.2e-7, as 0.5 (1 +
-// erff(x / sqrt 2)) is by 0.6e-7. At 5.4 x Q passes 0.5, so that larger |x|
-// give exactly x or 0. All but four operations of a pair are packed: 10.5
-// issue slots a value, half of CUDA's erff in the same formula, which
-// bounded the epilogue of the 8-bit product.
+// Exact GELU, x Phi(x), of two values. Phi(x) = 0.5 + x Q(min(x^2, X^2)),
+// clamped to 0..1, where Q is the polynomial in s = 2 x^2 / X^2 - 1 with the
+// least largest error of x Q over |x| <= X (fitted here in 64 bits). FINE:
+// degree 14, X = 5.4, and Phi off by at most 1.3e-7 in float32 arithmetic, as 0.5
+// (1 + erff(x / sqrt 2)) is by 0.6e-7; otherwise degree 12, X = 5.2, 4.3e-7,
+// which is for results that are rounded to bfloat16 (2^-8). At X, x Q passes
+// 0.5, so that larger |x| give exactly x or 0. In packed multiply-adds but for
+// four operations of a pair: about half the issue slots of CUDA's erff in
+// the same formula, which bounded the epilogue of the 8-bit product.
+template <bool FINE>
 __device__ __forceinline__ float2 gelu2(float2 x)
 {
-    constexpr float P[15] = {
-        0.26185622811317444f,   -0.13065610826015472f,  0.09699918329715729f,
-        -0.07841362804174423f,  0.0642331913113594f,    -0.05149291455745697f,
-        0.03929029032588005f,   -0.027926640585064888f, 0.01930239051580429f,
-        -0.01343067642301321f,  0.007317845709621906f,  -0.002372820395976305f,
-        0.0017498668748885393f, -0.0020567376632243395f, 0.0007857177406549454f};
+    constexpr int D = FINE ? 14 : 12;
+    constexpr float X = FINE ? 5.4f : 5.2f;
+    constexpr float Q14[15] = {
+        0.13092811405658722f,    -0.06532805413007736f,  0.04849959164857864f,
+        -0.03920681402087212f,   0.03211659565567970f,   -0.02574645727872848f,
+        0.01964514516294003f,    -0.01396332029253245f,  0.00965119525790214f,
+        -0.006715338211506605f,  0.003658922854810953f,  -0.0011864101979881525f,
+        0.0008749334374442696f,  -0.0010283688316121697f, 0.00039285887032747269f};
+    constexpr float Q12[13] = {
+        0.13594993948936462f,  -0.06774269789457321f,  0.05002840608358383f,
+        -0.03995957598090172f, 0.03193814679980278f,   -0.024464763700962067f,
+        0.01820363663136959f,  -0.013464033603668213f, 0.008026459254324436f,
+        -0.003071868559345603f, 0.002321982756257057f, -0.0026904314290732145f,
+        0.0010786805069074035f};
     float2 u = fma2(x, x, pair(0.0f));
-    u = make_float2(fminf(u.x, 5.4f * 5.4f), fminf(u.y, 5.4f * 5.4f));
-    const float2 s = fma2(u, pair(2.0f / (5.4f * 5.4f)), pair(-1.0f));
-    float2 q = pair(0.5f * P[14]);
+    u = make_float2(fminf(u.x, X * X), fminf(u.y, X * X));
+    const float2 s = fma2(u, pair(2.0f / (X * X)), pair(-1.0f));
+    float2 q = pair(FINE ? Q14[D] : Q12[D <= 12 ? D : 0]);
 #pragma unroll
-    for (int i = 13; i >= 0; i--)
-        q = fma2(q, s, pair(0.5f * P[i]));
+    for (int i = D - 1; i >= 0; i--)
+        q = fma2(q, s, pair(FINE ? Q14[i] : Q12[i <= 12 ? i : 0]));
     return fma2(x, make_float2(fma_sat(x.x, q.x, 0.5f), fma_sat(x.y, q.y, 0.5f)), pair(0.0f));
 }
 
@@ -197,13 +207,13 @@ __device__ __forceinline__ float times_sigmoid(float v, float t)
     return __fdividef(v, 1.0f + __expf(-t));
 }
 
-// The activation of two values. GELU_TANH is v sigmoid(2 y) with y the
-// argument of its tanh.
-template <int ACT>
+// The activation of two values, FINE as in gelu2. GELU_TANH is v sigmoid(2 y)
+// with y the argument of its tanh.
+template <int ACT, bool FINE>
 __device__ __forceinline__ float2 act2(float2 v, float slope)
 {
     if (ACT == ACT_GELU)
-        return gelu2(v);
+        return gelu2<FINE>(v);
     if (ACT == ACT_RELU)
         return make_float2(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f));
     if (ACT == ACT_LEAKY)
@@ -222,7 +232,7 @@ __device__ __forceinline__ float2 act2(float2 v, float slope)
 template <int ACT>
 __device__ __forceinline__ float act1(float v, float slope)
 {
-    return act2<ACT>(make_float2(v, 0.0f), slope).x;
+    return act2<ACT, true>(make_float2(v, 0.0f), slope).x;
 }
 
 // The same with the activation known at run time only.

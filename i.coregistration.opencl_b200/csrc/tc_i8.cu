@@ -10,11 +10,11 @@
 //               128-byte swizzled, into a ring of STAGES;
 //   warp 1      tensor memory and MMA: four tcgen05.mma.kind::i8 (K = 32 each)
 //               per stage into one of two accumulators (tiles alternate);
-//   warps 2..9  epilogue, two per TMEM lane quadrant: a lane is a row, 32
+//   warps 2..17 epilogue, four per TMEM lane quadrant: a lane is a row, 16
 //               sums at a time through scales, bias, activation and residual
 //               into a swizzled block that a TMA store writes (clipped at
 //               the matrix's edge); rows that no tensor map can describe go
-//               out through the same block, a row per warp store.
+//               out through the same block.
 // Bytes of a row behind K, rows behind M and N: outside the tensor maps,
 // which read them as zeros. Every mbarrier wait is bounded (tc_common.cuh).
 
@@ -26,7 +26,12 @@ namespace tc {
 namespace {
 
 constexpr int BM = 128, BK = 128; // BK in bytes
-constexpr int NTHREADS = 320, EPI_WARPS = 8;
+// Sixteen epilogue warps, four to a scheduler: with eight (two) the latencies
+// of their chain (scales, TMEM, activation, staging) bound the kernel, 10.8
+// thousand cycles a 128 x 256 tile with GELU against 4.3 of its products.
+constexpr int EPI_WARPS = 16, NTHREADS = 64 + 32 * EPI_WARPS;
+// Bytes of an output block's row: 16 columns of float, 32 of bfloat16.
+constexpr int ROW = 64;
 
 struct Params {
     I8Gemm g;
@@ -35,6 +40,8 @@ struct Params {
     // passes a row's end wrote the rest of its last 16 bytes too (measured),
     // so that the last columns go out without the tensor map.
     int clean;
+    int al;   // sb and bias are 16-byte aligned
+    int al_r; // rows of R are
 };
 
 template <int BN>
@@ -46,7 +53,7 @@ template <int BN>
 struct Smem {
     alignas(1024) unsigned char a[stages<BN>()][BM * BK];
     alignas(1024) unsigned char b[stages<BN>()][BN * BK];
-    alignas(1024) unsigned char cst[EPI_WARPS][4096];
+    alignas(1024) unsigned char cst[EPI_WARPS][32 * ROW];
     uint64_t full[stages<BN>()], empty[stages<BN>()], acc_full[2], acc_empty[2];
     uint32_t tmem;
 };
@@ -68,13 +75,14 @@ __device__ __forceinline__ void mma_i8(uint32_t tmem, uint64_t da, uint64_t db, 
                  "l"(da), "l"(db), "r"(idesc), "r"(accum));
 }
 
-// The 32 columns of p from col on, zero behind n.
-__device__ __forceinline__ void load_cols(float v[32], const float *p, int col, int n)
+// The 16 columns of p from col on, zero behind n; whole: they exist and are
+// 16-byte aligned.
+__device__ __forceinline__ void load_cols(float v[16], const float *p, int col, int n, bool whole)
 {
     p += col;
-    if (col + 32 <= n && ((uintptr_t)p & 15) == 0) {
+    if (whole) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
+        for (int j = 0; j < 16; j += 4) {
             const float4 x = __ldg((const float4 *)(p + j));
             v[j] = x.x;
             v[j + 1] = x.y;
@@ -84,88 +92,174 @@ __device__ __forceinline__ void load_cols(float v[32], const float *p, int col, 
         return;
     }
 #pragma unroll
-    for (int j = 0; j < 32; j++)
+    for (int j = 0; j < 16; j++)
         v[j] = col + j < n ? __ldg(p + j) : 0.0f;
 }
 
-// v[j] += R[j] for the j < n (at most 32) columns of a residual row. (Not
-// through the read-only cache: R may be C.)
-__device__ __forceinline__ void add_row(float v[32], const float *R, int n)
+// The 16 values of a residual row from R on, zero behind n; whole: they exist
+// and are 16-byte aligned. (Not through the read-only cache: R may be C.)
+__device__ __forceinline__ void load_row(float v[16], const float *R, int n, bool whole)
 {
-    if (n >= 32 && ((uintptr_t)R & 15) == 0) {
+    if (whole) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
+        for (int j = 0; j < 16; j += 4) {
             const float4 x = *(const float4 *)(R + j);
-            v[j] += x.x;
-            v[j + 1] += x.y;
-            v[j + 2] += x.z;
-            v[j + 3] += x.w;
+            v[j] = x.x;
+            v[j + 1] = x.y;
+            v[j + 2] = x.z;
+            v[j + 3] = x.w;
         }
         return;
     }
 #pragma unroll
-    for (int j = 0; j < 32; j++)
-        if (j < n)
-            v[j] += R[j];
+    for (int j = 0; j < 16; j++)
+        v[j] = j < n ? R[j] : 0.0f;
 }
 
-__device__ __forceinline__ void add_row(float v[32], const __nv_bfloat16 *R, int n)
+__device__ __forceinline__ void load_row(float v[16], const __nv_bfloat16 *R, int n, bool whole)
 {
-    if (n >= 32 && ((uintptr_t)R & 15) == 0) {
+    if (whole) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 8) {
+        for (int j = 0; j < 16; j += 8) {
             const uint4 x = *(const uint4 *)(R + j);
             const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                v[j + 2 * k] += __uint_as_float(w[k] << 16);
-                v[j + 2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
+                v[j + 2 * k] = __uint_as_float(w[k] << 16);
+                v[j + 2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
             }
         }
         return;
     }
 #pragma unroll
-    for (int j = 0; j < 32; j++)
-        if (j < n)
-            v[j] += __bfloat162float(R[j]);
+    for (int j = 0; j < 16; j++)
+        v[j] = j < n ? __bfloat162float(R[j]) : 0.0f;
 }
 
-// Row l of a block of 32 columns in its tensor map's layout: rows of 128
-// bytes (float; 16-byte chunk c at c ^ (l % 8)) or of 64 (bfloat16; c ^ ((l /
-// 2) % 4)).
-__device__ __forceinline__ void stage_row(unsigned char *blk, int l, const float v[32], float *)
+// Address of 16-byte chunk c of row l of an output block, in its tensor map's
+// 64-byte swizzle.
+__device__ __forceinline__ unsigned char *chunk(unsigned char *blk, int l, int c)
+{
+    return blk + l * ROW + ((c ^ ((l >> 1) & 3)) << 4);
+}
+
+// 16 values of row l into a block, the h-th 16 of the row.
+__device__ __forceinline__ void stage_row(unsigned char *blk, int l, int, const float v[16], float *)
 {
 #pragma unroll
-    for (int c = 0; c < 8; c++)
-        *(float4 *)(blk + l * 128 + ((c ^ (l & 7)) << 4)) =
-            make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+    for (int c = 0; c < 4; c++)
+        *(float4 *)chunk(blk, l, c) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
 }
 
-__device__ __forceinline__ void stage_row(unsigned char *blk, int l, const float v[32],
+__device__ __forceinline__ void stage_row(unsigned char *blk, int l, int h, const float v[16],
                                           __nv_bfloat16 *)
 {
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
+    for (int c = 0; c < 2; c++) {
         uint32_t w[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * c + 2 * k], v[8 * c + 2 * k + 1]);
-            w[k] = *(const uint32_t *)&h;
+            const __nv_bfloat162 x = __floats2bfloat162_rn(v[8 * c + 2 * k], v[8 * c + 2 * k + 1]);
+            w[k] = *(const uint32_t *)&x;
         }
-        *(uint4 *)(blk + l * 64 + ((c ^ ((l >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        *(uint4 *)chunk(blk, l, 2 * h + c) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
-// Element (l, j) of such a block.
-__device__ __forceinline__ float staged(const unsigned char *blk, int l, int j, float *)
+// First k-block of tile t: tiles that share rows of A or of B begin their
+// depth at different blocks, so that the CTAs running at one time do not all
+// ask L2 for the same lines (the sums are integers: no order changes them).
+__device__ __forceinline__ int first_block(int t, int tiles_m, int nk)
 {
-    return *(const float *)(blk + l * 128 + (((j >> 2) ^ (l & 7)) << 4) + (j & 3) * 4);
+    return (int)(((unsigned)(t % tiles_m) * 5u + (unsigned)(t / tiles_m) * 3u) % (unsigned)nk);
 }
 
-__device__ __forceinline__ __nv_bfloat16 staged(const unsigned char *blk, int l, int j,
-                                                __nv_bfloat16 *)
+// One epilogue warp's part of a tile: TMEM lanes 32 q .. (rows of the tile from
+// m0 on) and the blocks part, part + 4, ... of columns (from n0 on) of the
+// accumulator acc, which is complete when `full` turns `parity`. Returns false
+// when that wait ran out; else the warp's reads of the accumulator are done.
+template <int BN, int ACT, typename TC>
+__device__ __forceinline__ bool tile_out(const Params &p, const CUtensorMap *tma_c,
+                                         unsigned char *cst, uint32_t acc, uint64_t *full,
+                                         uint32_t parity, int m0, int n0, int q, int part,
+                                         int lane)
 {
-    return *(const __nv_bfloat16 *)(blk + l * 64 + (((j >> 3) ^ ((l >> 1) & 3)) << 4) + (j & 7) * 2);
+    constexpr int COLS = ROW / (int)sizeof(TC); // of a block
+    const I8Gemm &g = p.g;
+    TC *C = (TC *)g.C;
+    const TC *R = (const TC *)g.R;
+    m0 += 32 * q;
+    const int row = m0 + lane;
+    const float sa = row < g.M ? __ldg(g.sa + row) : 0.0f;
+    constexpr int STEP = COLS * (EPI_WARPS / 4);
+    // The residual into L2 while the products run: read in place its lines
+    // came from memory one block after the other (15 thousand cycles of
+    // epilogue for a 128 x 256 float tile, 6 without a residual).
+    if (R && row < g.M)
+        for (int c0 = COLS * part; c0 < BN && n0 + c0 < g.N; c0 += STEP)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(R + (long)row * g.ldc + n0 + c0));
+    // Decided per warp: the TMEM loads below are warp-collective.
+    if (!__all_sync(0xffffffffu, mbar_wait(full, parity, 63)))
+        return false;
+    fence_after();
+    acc += (uint32_t)(32 * q) << 16;
+    const bool whole = p.al && n0 + BN <= g.N;
+    for (int c0 = COLS * part; c0 < BN && n0 + c0 < g.N; c0 += STEP) {
+        const int col = n0 + c0;
+        // The previous store has read the block.
+        if (lane == 0)
+            bulk_wait_read<0>();
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < COLS / 16; h++) {
+            const int at = col + 16 * h;
+            float v[16], sb[16], bias[16], r[16];
+            if (R && row < g.M)
+                load_row(r, R + (long)row * g.ldc + at, g.N - at, whole && p.al_r);
+            load_cols(sb, g.sb, at, g.N, whole);
+            if (g.bias)
+                load_cols(bias, g.bias, at, g.N, whole);
+            tmem_ld16(acc + c0 + 16 * h, v);
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+                // The token's scale first (see scaled() in linear_i8.cu).
+                const float2 y = fma2(make_float2(__int2float_rn(__float_as_int(v[j])),
+                                                  __int2float_rn(__float_as_int(v[j + 1]))),
+                                      pair(sa), pair(0.0f));
+                const float2 x = act2<ACT, sizeof(TC) == 4>(
+                    fma2(y, make_float2(sb[j], sb[j + 1]),
+                         g.bias ? make_float2(bias[j], bias[j + 1]) : pair(0.0f)),
+                    g.slope);
+                v[j] = x.x;
+                v[j + 1] = x.y;
+            }
+            if (R && row < g.M)
+#pragma unroll
+                for (int j = 0; j < 16; j++)
+                    v[j] += r[j];
+            stage_row(cst, lane, h, v, (TC *)nullptr);
+        }
+        if (p.tma_out && (col + COLS <= g.N || p.clean)) {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                tma_store_2d(tma_c, cst, col, m0);
+                bulk_commit();
+            }
+            continue;
+        }
+        __syncwarp();
+        // Rows without a tensor map: 32 / COLS rows at a time, lane = column.
+        const int c = lane % COLS;
+        if (col + c < g.N)
+            for (int r = lane / COLS; r < 32 && m0 + r < g.M; r += 32 / COLS)
+                C[(long)(m0 + r) * g.ldc + col + c] =
+                    ((const TC *)chunk(cst, r, c * (int)sizeof(TC) / 16))[c % (16 / (int)sizeof(TC))];
+    }
+    // Each tcgen05.ld has waited: the accumulator may be written again.
+    fence_before();
+    __syncwarp();
+    return true;
 }
 
 template <int BN, int ACT, typename TC>
@@ -207,7 +301,9 @@ tc_i8_k(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUten
             bool ok = true;
             for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
                 const int m0 = (t % tiles_m) * BM, n0 = (t / tiles_m) * BN;
-                for (int kb = 0; kb < nk; kb++, it++) {
+                const int off = first_block(t, tiles_m, nk);
+                for (int k = 0; k < nk; k++, it++) {
+                    const int kb = k + off < nk ? k + off : k + off - nk;
                     const int st = it % ST;
                     if (it >= ST && !mbar_wait(&s.empty[st], ((it / ST) - 1) & 1, 61)) {
                         ok = false;
@@ -250,69 +346,14 @@ tc_i8_k(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUten
         }
     }
     else {
-        // Warp w: TMEM lanes 32 (w % 4) .., the 32-column chunks of parity (w -
-        // 2) / 4.
-        const int q = warp % 4, half = (warp - 2) / 4;
         unsigned char *cst = s.cst[warp - 2];
-        TC *C = (TC *)g.C;
-        const TC *R = (const TC *)g.R;
         int lt = 0;
         for (int t = blockIdx.x; t < ntiles; t += gridDim.x, lt++) {
-            const int buf = lt % 2, use = lt / 2;
-            const int m0 = (t % tiles_m) * BM + 32 * q, n0 = (t / tiles_m) * BN;
-            const int row = m0 + lane;
-            const float sa = row < g.M ? __ldg(g.sa + row) : 0.0f;
-            // Decided per warp: the TMEM loads below are warp-collective.
-            if (!__all_sync(0xffffffffu, mbar_wait_backoff(&s.acc_full[buf], use & 1, 63)))
+            const int buf = lt % 2;
+            if (!tile_out<BN, ACT, TC>(p, &tma_c, cst, tmem + (uint32_t)(buf * acc_cols<BN>()),
+                                       &s.acc_full[buf], lt / 2 & 1, (t % tiles_m) * BM,
+                                       (t / tiles_m) * BN, warp % 4, (warp - 2) / 4, lane))
                 break;
-            fence_after();
-            const uint32_t acc =
-                tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(buf * acc_cols<BN>());
-            for (int c0 = 32 * half; c0 < BN && n0 + c0 < g.N; c0 += 64) {
-                const int col = n0 + c0;
-                float v[32], sb[32], bias[32];
-                load_cols(sb, g.sb, col, g.N);
-                if (g.bias)
-                    load_cols(bias, g.bias, col, g.N);
-                tmem_ld32(acc + c0, v);
-#pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                    // The token's scale first (see scaled() in linear_i8.cu).
-                    const float2 y = fma2(make_float2(__int2float_rn(__float_as_int(v[j])),
-                                                      __int2float_rn(__float_as_int(v[j + 1]))),
-                                          pair(sa), pair(0.0f));
-                    const float2 x = act2<ACT>(
-                        fma2(y, make_float2(sb[j], sb[j + 1]),
-                             g.bias ? make_float2(bias[j], bias[j + 1]) : pair(0.0f)),
-                        g.slope);
-                    v[j] = x.x;
-                    v[j + 1] = x.y;
-                }
-                if (R && row < g.M)
-                    add_row(v, R + (long)row * g.ldc + col, g.N - col);
-                // The previous store has read the staging block.
-                if (lane == 0)
-                    bulk_wait_read<0>();
-                __syncwarp();
-                stage_row(cst, lane, v, (TC *)nullptr);
-                if (p.tma_out && (col + 32 <= g.N || p.clean)) {
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        tma_store_2d(&tma_c, cst, col, m0);
-                        bulk_commit();
-                    }
-                    continue;
-                }
-                __syncwarp();
-                if (col + lane < g.N)
-                    for (int r = 0; r < 32 && m0 + r < g.M; r++)
-                        C[(long)(m0 + r) * g.ldc + col + lane] = staged(cst, r, lane, (TC *)nullptr);
-            }
-            // This warp's reads of the accumulator are complete (each
-            // tcgen05.ld waited): hand it back to the MMA warp.
-            fence_before();
-            __syncwarp();
             if (lane == 0)
                 mbar_arrive(&s.acc_empty[buf]);
         }
@@ -349,8 +390,10 @@ bool launch(cudaStream_t st, const I8Gemm &g, int sms)
     if (!make_map_rows(&ma, g.A, 1, g.M, g.K, g.lda, BK, BM, 128) ||
         !make_map_rows(&mb, g.B, 1, g.N, g.K, g.ldb, BK, BN, 128))
         return false;
-    p.tma_out = make_map_rows(&mc, g.C, sizeof(TC), g.M, g.N, g.ldc * (long)sizeof(TC), 32, 32,
-                              sizeof(TC) == 4 ? 128 : 64);
+    p.tma_out = make_map_rows(&mc, g.C, sizeof(TC), g.M, g.N, g.ldc * (long)sizeof(TC),
+                              ROW / (int)sizeof(TC), 32, 64);
+    p.al = (((uintptr_t)g.sb | (uintptr_t)g.bias) & 15) == 0;
+    p.al_r = ((uintptr_t)g.R & 15) == 0 && g.ldc * (long)sizeof(TC) % 16 == 0;
     p.clean = (long)g.N * (int)sizeof(TC) % 16 == 0;
     const long tiles = (long)cdiv(g.M, BM) * cdiv(g.N, BN);
     if (tiles >= (1L << 31))
@@ -374,13 +417,21 @@ bool launch(cudaStream_t st, const I8Gemm &g, int sms)
 template <typename TC>
 bool choose(cudaStream_t st, const I8Gemm &g, int sms)
 {
-    // The width whose tiles take the least time over their rounds of CTAs.
+    // The width whose tiles take the least time, in cycles: a round of tiles
+    // costs its products or, where that is more, its epilogue, and the last
+    // epilogue overlaps nothing. 128 bytes of depth take about 600 cycles at
+    // any width: an MMA reads its 128 rows of A for 128 cycles, in which it
+    // multiplies up to 256 columns (25616 x 4096 x 1024: 125 us with 256
+    // columns, 144 with 128, 231 with 64; 500 x 500 x 500, where rounds do
+    // not count: 13.5, 10.3 and 8.4).
     const int widths[3] = {256, 128, 64};
     int best = 0;
     double best_t = 0;
     for (int i = 0; i < 3; i++) {
-        const long tiles = (long)cdiv(g.M, BM) * cdiv(g.N, widths[i]);
-        const double t = (double)((tiles + sms - 1) / sms) * (widths[i] + 24);
+        const int bn = widths[i];
+        const long tiles = (long)cdiv(g.M, BM) * cdiv(g.N, bn), rounds = (tiles + sms - 1) / sms;
+        const double main = 600.0 * cdiv(g.K, BK), epi = 1500.0 + 20.0 * bn;
+        const double t = rounds * ((main > epi ? main : epi) + 500.0) + epi;
         if (i == 0 || t < best_t) {
             best = i;
             best_t = t;
