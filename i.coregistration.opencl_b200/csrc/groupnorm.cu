@@ -422,6 +422,8 @@ groupnorm_k(const __grid_constant__ GroupNorm p)
     // The row lane that holds the map's last super row, -1 if none here.
     const int last = sr1 == p.nsr && rows > 0 ? (more > 0 ? more : p.lanes) - 1 : -1;
 
+    if (!GRID)
+        after_previous();
     for (int img = GRID ? 0 : (int)blockIdx.y; img < p.nimg; img += GRID ? 1 : p.nimg) {
         const TX *x = (const TX *)p.X + img * p.sx + c0;
         TY *y = (TY *)p.Y + img * p.sy + c0;
@@ -786,7 +788,7 @@ bool launch(cudaStream_t st, GroupNorm p, int sms)
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     cfg.attrs = at;
     cfg.numAttrs = 1;
     if (best_grid) {
@@ -799,6 +801,9 @@ bool launch(cudaStream_t st, GroupNorm p, int sms)
         at[0].id = cudaLaunchAttributeClusterDimension;
         at[0].val.clusterDim.x = best.team;
         at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[1].val.programmaticStreamSerializationAllowed = 1; // (see after_previous)
+        cfg.numAttrs = 2;
     }
     void *args[] = {&best};
     cuda_ok(cudaLaunchKernelExC(&cfg, fn, args), "groupnorm_cl");

@@ -23,54 +23,50 @@ namespace {
 // exact in one fused multiply-add: x and s are multiples of the smaller of
 // their last places, and the difference is below s (in units of that place
 // below 2^24). So |x - q s| against s / 2 decides, without a division, and
-// the seldom value that it moves takes a branch.
+// the seldom values that it moves take a branch.
 struct RowScale {
     float s, inv, half;
-    bool tiny; // s below 2^-90: 1 / s could overflow, s could be denormal
     __device__ explicit RowScale(uint32_t amax)
     {
-        if (amax >= 0x7f800000u) {
-            s = __int_as_float(0x7fffffff);
-            inv = half = 0.0f;
-            tiny = false;
-            return;
+        s = __int_as_float(0x7fffffff);
+        inv = half = 0.0f;
+        if (amax < 0x7f800000u) {
+            s = __fdiv_rn(__uint_as_float(amax), 127.0f);
+            // Below 2^-90 1 / s could overflow and s be denormal: slow().
+            if (s >= 0x1p-90f) {
+                inv = __fdiv_rn(1.0f, s);
+                half = 0.5f * s;
+            }
         }
-        s = __fdiv_rn(__uint_as_float(amax), 127.0f);
-        tiny = s < 0x1p-90f;
-        inv = tiny ? 0.0f : __fdiv_rn(1.0f, s);
-        half = 0.5f * s;
     }
-    // The quantised value as the low byte of the result.
+    // The quantised value as the low byte of the result; sure: whether it is.
+    __device__ __forceinline__ uint32_t guess(float x, bool &sure) const
+    {
+        const float big = fmaf(x, inv, 12582912.0f);
+        const float d = fmaf(12582912.0f - big, s, x);
+        sure = sure && fabsf(d) < half;
+        return __float_as_uint(big);
+    }
+    // Any value of any row: next to a tie, or of a scale that is not a normal
+    // positive number.
+    __device__ __noinline__ uint32_t slow(float x) const
+    {
+        if (!(s > 0.0f))
+            return 0; // a row of zeros, or with an infinity or NaN
+        // Small scales into the normal range by an exact power of two.
+        const float k = s < 0x1p-90f ? 0x1p+90f : 1.0f, u = s * k;
+        x *= k;
+        float q = rintf(__fdiv_rn(x, u));
+        const float d = fmaf(-q, u, x), e = fabsf(d + d);
+        if (e > u || (e == u && ((int)q & 1)))
+            q += copysignf(1.0f, d);
+        return (uint32_t)(int)fminf(fmaxf(q, -127.0f), 127.0f);
+    }
     __device__ __forceinline__ uint32_t of(float x) const
     {
-        const float big = fmaf(x, inv, 12582912.0f), q = big - 12582912.0f;
-        const float d = fmaf(-q, s, x);
-        if (fabsf(d) < half)
-            return __float_as_uint(big);
-        return slow(x, q, d);
-    }
-    // Values next to a tie, and rows without a normal positive scale.
-    __device__ __noinline__ uint32_t slow(float x, float q, float d) const
-    {
-        if (tiny) {
-            // Into the normal range by an exact power of two.
-            const float up = s * 0x1p+90f;
-            if (!(up > 0.0f))
-                return 0;
-            x *= 0x1p+90f;
-            q = rintf(__fdiv_rn(x, up));
-            d = fmaf(-q, up, x);
-            const float e = fabsf(d + d);
-            if (e > up || (e == up && ((int)q & 1)))
-                q += copysignf(1.0f, d);
-        }
-        else if (!(s > 0.0f)) {
-            return 0; // a row with an infinity or NaN
-        }
-        else if (fabsf(d) > half || ((int)q & 1)) {
-            q += copysignf(1.0f, d);
-        }
-        return (uint32_t)(int)fminf(fmaxf(q, -127.0f), 127.0f);
+        bool sure = true;
+        const uint32_t q = guess(x, sure);
+        return sure ? q : slow(x);
     }
 };
 
@@ -103,11 +99,22 @@ struct Piece {
     }
     __device__ __forceinline__ void store(int8_t *q, const RowScale &s) const
     {
-        const uint32_t a = pack4(s.of(at(0)), s.of(at(1)), s.of(at(2)), s.of(at(3)));
-        if constexpr (V == 4)
-            *(uint32_t *)q = a;
-        else
-            *(uint2 *)q = make_uint2(a, pack4(s.of(at(4)), s.of(at(5)), s.of(at(6)), s.of(at(7))));
+        uint32_t v[V];
+        bool sure = true;
+#pragma unroll
+        for (int e = 0; e < V; e++)
+            v[e] = s.guess(at(e), sure);
+        if (!sure) {
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                v[e] = s.slow(at(e));
+        }
+        if constexpr (V == 4) {
+            *(uint32_t *)q = pack4(v[0], v[1], v[2], v[3]);
+        }
+        else {
+            *(uint2 *)q = make_uint2(pack4(v[0], v[1], v[2], v[3]), pack4(v[4], v[5], v[6], v[7]));
+        }
     }
 };
 
@@ -131,6 +138,7 @@ __global__ void __launch_bounds__(256)
 quant_k(const T *X, long ldx, long rows, int C, int8_t *Q, long ldq, float *S)
 {
     __shared__ uint32_t red[8];
+    after_previous();
     const int lane = threadIdx.x % G;
     const long row = (long)blockIdx.x * (256 / G) + threadIdx.x / G;
     const bool here = row < rows;
@@ -189,24 +197,24 @@ quant_k(const T *X, long ldx, long rows, int C, int8_t *Q, long ldq, float *S)
 template <typename T, int V>
 void quant_launch(cudaStream_t st, const View &x, int8_t *q, long ldq, float *s)
 {
-    // A warp per row up to 8 pieces a lane, then a quarter of a block, then a
+    // A warp per row up to 8 pieces a lane (no barrier of the block), then a
     // block.
     const int pieces = (int)(x.cols / V);
-    const T *p = (const T *)x.p;
     auto go = [&](auto g, auto np) {
         constexpr int G = decltype(g)::value, NP = decltype(np)::value;
-        quant_k<T, V, G, NP><<<cdiv(x.rows, 256 / G), 256, 0, st>>>(p, x.ld, x.rows, (int)x.cols, q,
-                                                                    ldq, s);
+        launch_chained(quant_k<T, V, G, NP>, cdiv(x.rows, 256 / G), 256, 0, st, (const T *)x.p, x.ld,
+                       x.rows, (int)x.cols, q, ldq, s);
     };
-    typedef std::integral_constant<int, 32> warp;
-    typedef std::integral_constant<int, 64> two;
-    typedef std::integral_constant<int, 256> block;
     typedef std::integral_constant<int, 4> four;
     typedef std::integral_constant<int, 8> eight;
+    typedef std::integral_constant<int, 32> warp;
+    typedef std::integral_constant<int, 256> block;
     if (pieces <= 32 * 4)
         go(warp(), four());
-    else if (pieces <= 64 * 4)
-        go(two(), four());
+    else if (pieces <= 32 * 8)
+        go(warp(), eight());
+    else if (pieces <= 256 * 4)
+        go(block(), four());
     else
         go(block(), eight());
 }
@@ -317,6 +325,7 @@ i8_skinny_k(const I8Gemm g)
     const int8_t *w0 = g.B + (long)min(n0 + r, g.N - 1) * g.ldb;
     const int8_t *w1 = g.B + (long)min(n0 + r + 8, g.N - 1) * g.ldb;
     int d[NT][4] = {};
+    after_previous();
     constexpr int U = NT == 4 ? 2 : 4, STEP = SK_WARPS * SK_TURN;
     for (int k0 = warp * SK_TURN + kk; k0 < g.K + kk; k0 += U * STEP) {
         uint4 a[U], b[U];
@@ -364,11 +373,11 @@ void skinny(cudaStream_t st, const I8Gemm &g)
 {
     const unsigned grid = cdiv(g.N, SK_CH);
     if (g.M <= 8)
-        i8_skinny_k<1, TC><<<grid, 32 * SK_WARPS, 0, st>>>(g);
+        launch_chained(i8_skinny_k<1, TC>, grid, 32 * SK_WARPS, 0, st, g);
     else if (g.M <= 16)
-        i8_skinny_k<2, TC><<<grid, 32 * SK_WARPS, 0, st>>>(g);
+        launch_chained(i8_skinny_k<2, TC>, grid, 32 * SK_WARPS, 0, st, g);
     else
-        i8_skinny_k<4, TC><<<grid, 32 * SK_WARPS, 0, st>>>(g);
+        launch_chained(i8_skinny_k<4, TC>, grid, 32 * SK_WARPS, 0, st, g);
 }
 
 constexpr int SKINNY_ROWS = 32;

@@ -130,7 +130,37 @@ inline bool same_view(const View &a, const View &b)
 // Multiprocessors of the backend's device.
 inline int sms_of(const struct ocl_backend *ocl) { return ocl->sm_count > 0 ? ocl->sm_count : 148; }
 
+// Launches a kernel whose blocks may start while the stream's previous kernel
+// ends (programmatic stream serialization): every thread of it calls
+// after_previous() before its first access to global memory.
+template <typename... P, typename... A>
+bool launch_chained(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem,
+                    cudaStream_t st, const A &...args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cuda_ok(cudaLaunchKernelEx(&cfg, kernel, P(args)...), "kernel launch");
+}
+
 }  // namespace coreg
+
+// Lets the stream's next kernel start its blocks as this one's leave room (it
+// waits in its own after_previous), then waits until the previous kernel has
+// ended and its writes are visible. Saves the launch latency between
+// dependent kernels, 1 to 2 us.
+__device__ __forceinline__ void after_previous()
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 
 // ------------------------------------------------------------ activations
 

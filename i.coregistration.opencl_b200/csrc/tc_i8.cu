@@ -290,6 +290,7 @@ tc_i8_k(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUten
     }
     if (warp == 1)
         tmem_alloc(&s.tmem, 2 * acc_cols<BN>());
+    after_previous();
     fence_before();
     __syncthreads();
     fence_after();
@@ -377,7 +378,7 @@ bool run(cudaStream_t st, int grid, const CUtensorMap &ma, const CUtensorMap &mb
     static unsigned done = 0;
     if (!smem_opt_in((const void *)tc_i8_k<BN, ACT, TC>, smem, &done))
         return false;
-    tc_i8_k<BN, ACT, TC><<<grid, NTHREADS, smem, st>>>(ma, mb, mc, p);
+    launch_chained(tc_i8_k<BN, ACT, TC>, grid, NTHREADS, smem, st, ma, mb, mc, p);
     return true;
 }
 
