@@ -314,7 +314,7 @@ __device__ __forceinline__ void apply(const GroupNorm &p, const TX *x, TY *y, co
         else {
 #pragma unroll
             for (int e = 0; e < V; e += 2) {
-                const float2 v = act2<ACT, sizeof(TY) == 4>(make_float2(fmaf(r.at(e) - mean[e], a[e], b[e]),
+                const float2 v = act2<ACT>(make_float2(fmaf(r.at(e) - mean[e], a[e], b[e]),
                                                        fmaf(r.at(e + 1) - mean[e + 1], a[e + 1],
                                                             b[e + 1])),
                                            p.slope);

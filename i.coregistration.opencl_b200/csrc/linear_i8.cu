@@ -282,114 +282,384 @@ i8_tile_k(const I8Gemm g)
         }
 }
 
-// Few rows: the weights stream once from memory, so a block takes 16 of
-// their rows (output channels), its 8 warps the depth by turns of 64 bytes.
-// mma.m16n8k32 of 8-bit integers with the weights as the 16 rows and 8 tokens
-// as the columns: lane l's operands are four words of channel (or token) l /
-// 4, and as the order of the depth is free as long as both operands agree,
-// they are one 16-byte load at 16 (l % 4) of the turn. The warps' sums meet
-// in shared memory.
-constexpr int SK_CH = 16, SK_WARPS = 8, SK_TURN = 64;
+// Few tokens: the weights stream once from memory. A warp takes 16 of their
+// rows (output channels) in steps of 64 bytes of depth; for deep and narrow
+// layers `split` warps share a row's depth. The products go through
+// mma.m16n8k16 of float16 with the weights as the 16 rows and 8 tokens as the
+// columns: 8-bit integers are exact in float16, their products and sums of
+// 256 of them (at most 2^22) in float32, and are added up as integers from
+// there. Lane l's operands are those of channel (or token) l / 4, and as the
+// order of the depth is free as long as both operands agree, they are one
+// 16-byte load at 16 (l % 4) of the step. (The integer forms are slow here:
+// mma.sync of 8-bit integers took 150 cycles and more, __dp4a runs at 8 per
+// cycle and multiprocessor; 8192 x 8192 with 8 tokens 63 us with it.)
+constexpr int FEW_WARPS = 8, FEW_CH = 16, FEW_STEP = 64;
 
-__device__ __forceinline__ void mma_s8(int d[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                       uint32_t a3, uint32_t b0, uint32_t b1)
+__device__ __forceinline__ void mma_f16(float d[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
                  "{%8,%9}, {%0,%1,%2,%3};"
-                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Four 8-bit integers as float16 pairs: x + 128 as the low byte of 1024 (0x6400)
+// is 1152 + x, from which 1152 is taken off.
+__device__ __forceinline__ void halves(uint32_t w, uint32_t &lo, uint32_t &hi)
+{
+    w ^= 0x80808080u;
+    lo = __byte_perm(w, 0x64646464u, 0x4140);
+    hi = __byte_perm(w, 0x64646464u, 0x4342);
+    asm("sub.f16x2 %0, %0, %1;" : "+r"(lo) : "r"(0x64806480u));
+    asm("sub.f16x2 %0, %0, %1;" : "+r"(hi) : "r"(0x64806480u));
 }
 
 // 16 bytes of a row from depth k on, zeros behind K: the bytes there need not
 // exist.
-__device__ __forceinline__ uint4 load16(const int8_t *row, int k, int K)
+__device__ __noinline__ uint4 load_end(const int8_t *p, int n)
 {
-    if (k + 16 <= K)
-        return *(const uint4 *)(row + k);
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 16; i++)
-        if (k + i < K)
-            w[i / 4] |= (uint32_t)(uint8_t)row[k + i] << (8 * (i % 4));
+        if (i < n)
+            w[i / 4] |= (uint32_t)(uint8_t)p[i] << (8 * (i % 4));
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// NT: groups of 8 tokens.
-template <int NT, typename TC>
-__global__ void __launch_bounds__(32 * SK_WARPS)
-i8_skinny_k(const I8Gemm g)
+__device__ __forceinline__ uint4 load16(const int8_t *row, int k, int K)
 {
-    __shared__ int part[SK_WARPS][SK_CH][8 * NT + 1];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, n0 = blockIdx.x * SK_CH;
-    const int r = lane / 4, kk = 16 * (lane % 4);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (k + 16 <= K)
+        v = *(const uint4 *)(row + k);
+    else if (k < K)
+        v = load_end(row + k, K - k);
+    return v;
+}
+
+// Tokens that the kernel quantises itself (ops_linear_i8): each block all of
+// them, into shared memory, while its first weights are on their way.
+struct Tokens {
+    const void *X;
+    long ldx;
+    int pitch; // bytes of a quantised row
+};
+
+int token_pitch(int K) { return (K + 15) / 16 * 16; }
+
+// The M rows of x quantised as by ops_quant_i8 into q, scales into s; amax: M
+// words, zero. Ends with a barrier.
+template <typename T>
+__device__ void quant_tokens(const Tokens &x, int M, int K, int8_t *q, float *s, uint32_t *amax)
+{
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    // Warps of a row: 8 of one, 4 of two, 2 of four, then a warp per row.
+    const int per = M == 1 ? 8 : M == 2 ? 4 : M <= 4 ? 2 : 1, sub = warp % per;
+    const int V = 16 / (int)sizeof(T);
+    const bool al = ((uintptr_t)x.X & 15) == 0 && (M == 1 || x.ldx % V == 0);
+    const int whole = al ? K / V * V : 0; // columns taken V at a time
+    for (int r = warp / per; r < M; r += FEW_WARPS / per) {
+        const T *p = (const T *)x.X + r * x.ldx;
+        uint32_t m = 0;
+        for (int c = (sub * 32 + lane) * V; c < whole; c += per * 32 * V) {
+            Piece<T, V> f;
+            f.load(p + c);
+            m = max(m, f.top());
+        }
+        for (int c = whole + sub * 32 + lane; c < K; c += per * 32)
+            m = max(m, magnitude(ldf(p + c)));
+        m = __reduce_max_sync(0xffffffffu, m);
+        if (lane == 0)
+            atomicMax(&amax[r], m); // (the largest, in whatever order)
+    }
+    __syncthreads();
+    for (int r = warp / per; r < M; r += FEW_WARPS / per) {
+        const T *p = (const T *)x.X + r * x.ldx;
+        int8_t *to = q + r * x.pitch;
+        const RowScale rs(amax[r]);
+        if (sub == 0 && lane == 0)
+            s[r] = rs.s;
+        for (int c = (sub * 32 + lane) * V; c < whole; c += per * 32 * V) {
+            Piece<T, V> f;
+            f.load(p + c);
+            f.store(to + c, rs);
+        }
+        // One by one, with zeros up to the end of the pitch.
+        for (int c = whole + sub * 32 + lane; c < x.pitch; c += per * 32)
+            to[c] = c < K ? (int8_t)rs.of(ldf(p + c)) : (int8_t)0;
+    }
+    __syncthreads();
+}
+
+// NT: groups of 8 tokens. TX: the type of tokens that come unquantised (the
+// struct x; then g.A and g.sa are not used), or void.
+template <int NT, typename TC, typename TX>
+__global__ void __launch_bounds__(32 * FEW_WARPS)
+i8_few_k(const I8Gemm g, const Tokens x, int split)
+{
+    constexpr bool FLOATS = !std::is_same<TX, void>::value;
+    constexpr int THREADS = 32 * FEW_WARPS;
+    __shared__ int part[FEW_WARPS][FEW_CH][8 * NT + 1];
+    __shared__ float scale[8 * NT];
+    __shared__ uint32_t amax[8 * NT];
+    extern __shared__ __align__(16) int8_t tok[];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int channels = FEW_WARPS / split * FEW_CH, c0 = blockIdx.x * channels;
+    const int n0 = c0 + warp / split * FEW_CH, r = lane / 4, kk = 16 * (lane % 4);
+    if (FLOATS && threadIdx.x < 8 * NT)
+        amax[threadIdx.x] = 0;
+    after_previous();
     const int8_t *w0 = g.B + (long)min(n0 + r, g.N - 1) * g.ldb;
     const int8_t *w1 = g.B + (long)min(n0 + r + 8, g.N - 1) * g.ldb;
-    int d[NT][4] = {};
-    after_previous();
-    constexpr int U = NT == 4 ? 2 : 4, STEP = SK_WARPS * SK_TURN;
-    for (int k0 = warp * SK_TURN + kk; k0 < g.K + kk; k0 += U * STEP) {
-        uint4 a[U], b[U];
+    // Four steps at a time, the next four's weights under way.
+    constexpr int U = 4;
+    const int step = split * FEW_STEP;
+    int k = (warp % split) * FEW_STEP + kk;
+    uint4 a[U], b[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        a[u] = load16(w0, k + u * step, g.K);
+        b[u] = load16(w1, k + u * step, g.K);
+    }
+    // The epilogue's thread: channel c, tokens m0, m0 + THREADS / channels, ...
+    const int c = threadIdx.x % channels, m0 = threadIdx.x / channels;
+    const bool out = c0 + c < g.N;
+    const float sb = out ? __ldg(g.sb + c0 + c) : 0.0f;
+    const float bias = out && g.bias ? __ldg(g.bias + c0 + c) : 0.0f;
+    if constexpr (FLOATS) {
+        __syncthreads();
+        quant_tokens<TX>(x, g.M, g.K, tok, scale, amax);
+    }
+    else if (threadIdx.x < g.M) {
+        scale[threadIdx.x] = __ldg(g.sa + threadIdx.x);
+    }
+    int sum[NT][4] = {};
+    for (; k - kk < g.K; k += U * step) {
+        float d[NT][4] = {};
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            a[u] = load16(w0, k0 + u * STEP, g.K);
-            b[u] = load16(w1, k0 + u * STEP, g.K);
-        }
-#pragma unroll
-        for (int u = 0; u < U; u++)
+            uint4 v[NT];
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-                const int m = 8 * t + r;
-                const uint4 x = m < g.M ? load16(g.A + (long)m * g.lda, k0 + u * STEP, g.K)
-                                        : make_uint4(0, 0, 0, 0);
-                mma_s8(d[t], a[u].x, b[u].x, a[u].y, b[u].y, x.x, x.y);
-                mma_s8(d[t], a[u].z, b[u].z, a[u].w, b[u].w, x.z, x.w);
+                const int m = 8 * t + r, at = k + u * step;
+                v[t] = make_uint4(0, 0, 0, 0);
+                if (m < g.M) {
+                    if (!FLOATS)
+                        v[t] = load16(g.A + (long)m * g.lda, at, g.K);
+                    else if (at < g.K)
+                        v[t] = *(const uint4 *)(tok + m * x.pitch + at);
+                }
             }
+            const uint32_t wa[4] = {a[u].x, a[u].y, a[u].z, a[u].w};
+            const uint32_t wb[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint32_t a0, a1, a2, a3;
+                halves(wa[i], a0, a2);
+                halves(wb[i], a1, a3);
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    uint32_t b0, b1;
+                    halves(i == 0 ? v[t].x : i == 1 ? v[t].y : i == 2 ? v[t].z : v[t].w, b0, b1);
+                    mma_f16(d[t], a0, a1, a2, a3, b0, b1);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            a[u] = load16(w0, k + (U + u) * step, g.K);
+            b[u] = load16(w1, k + (U + u) * step, g.K);
+        }
+        // U steps are 256 of depth.
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                sum[t][i] += __float2int_rn(d[t][i]);
     }
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            part[warp][r + 8 * (i / 2)][8 * t + 2 * (lane % 4) + i % 2] = d[t][i];
+            part[warp][r + 8 * (i / 2)][8 * t + 2 * (lane % 4) + i % 2] = sum[t][i];
     __syncthreads();
-    for (int e = threadIdx.x; e < SK_CH * g.M; e += 32 * SK_WARPS) {
-        const int c = e % SK_CH, m = e / SK_CH;
-        if (n0 + c >= g.N)
-            continue;
-        int acc = 0;
-#pragma unroll
-        for (int w = 0; w < SK_WARPS; w++)
-            acc += part[w][c][m];
-        float v = scaled(acc, g.sa[m], g.sb[n0 + c], g.bias ? g.bias[n0 + c] : 0.0f);
-        v = act_any(v, g.act, g.slope);
-        const long at = (long)m * g.ldc + n0 + c;
+    if (!out)
+        return;
+    for (int m = m0; m < g.M; m += THREADS / channels) {
+        int s = 0;
+        for (int i = 0; i < split; i++)
+            s += part[c / FEW_CH * split + i][c % FEW_CH][m];
+        float v = act_any(scaled(s, scale[m], sb, bias), g.act, g.slope);
+        const long at = (long)m * g.ldc + c0 + c;
         if (g.R)
             v += ldf((const TC *)g.R + at);
         stf((TC *)g.C + at, v);
     }
 }
 
-template <typename TC>
-void skinny(cudaStream_t st, const I8Gemm &g)
+// One or two tokens: a warp takes ROWS rows of the weights, its lanes 16 bytes of
+// depth each, 512 bytes of a row together; four products per __dp4a, the lanes'
+// sums in one reduction instruction each. `split` as above.
+constexpr int DOT_ROWS = 4, DOT_STEP = 512;
+
+template <int MT, typename TC, typename TX>
+__global__ void __launch_bounds__(32 * FEW_WARPS)
+i8_dot_k(const I8Gemm g, const Tokens x, int split)
 {
-    const unsigned grid = cdiv(g.N, SK_CH);
-    if (g.M <= 8)
-        launch_chained(i8_skinny_k<1, TC>, grid, 32 * SK_WARPS, 0, st, g);
-    else if (g.M <= 16)
-        launch_chained(i8_skinny_k<2, TC>, grid, 32 * SK_WARPS, 0, st, g);
-    else
-        launch_chained(i8_skinny_k<4, TC>, grid, 32 * SK_WARPS, 0, st, g);
+    constexpr bool FLOATS = !std::is_same<TX, void>::value;
+    constexpr int THREADS = 32 * FEW_WARPS, U = 2;
+    __shared__ int part[FEW_WARPS][DOT_ROWS][MT];
+    __shared__ float scale[MT];
+    __shared__ uint32_t amax[MT];
+    extern __shared__ __align__(16) int8_t tok[];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int channels = FEW_WARPS / split * DOT_ROWS, c0 = blockIdx.x * channels;
+    const int n0 = c0 + warp / split * DOT_ROWS;
+    if (FLOATS && threadIdx.x < MT)
+        amax[threadIdx.x] = 0;
+    after_previous();
+    const int8_t *w[DOT_ROWS];
+#pragma unroll
+    for (int r = 0; r < DOT_ROWS; r++)
+        w[r] = g.B + (long)min(n0 + r, g.N - 1) * g.ldb;
+    const int step = split * DOT_STEP;
+    int k = (warp % split) * DOT_STEP + 16 * lane;
+    uint4 a[U][DOT_ROWS];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int r = 0; r < DOT_ROWS; r++)
+            a[u][r] = load16(w[r], k + u * step, g.K);
+    const int c = threadIdx.x % channels, m0 = threadIdx.x / channels;
+    const bool out = m0 < g.M && c0 + c < g.N;
+    const float sb = out ? __ldg(g.sb + c0 + c) : 0.0f;
+    const float bias = out && g.bias ? __ldg(g.bias + c0 + c) : 0.0f;
+    if constexpr (FLOATS) {
+        __syncthreads();
+        quant_tokens<TX>(x, g.M, g.K, tok, scale, amax);
+    }
+    else if (threadIdx.x < g.M) {
+        scale[threadIdx.x] = __ldg(g.sa + threadIdx.x);
+    }
+    int acc[DOT_ROWS][MT] = {};
+    for (; k - 16 * lane < g.K; k += U * step) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int at = k + u * step;
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (m < g.M) {
+                    if (!FLOATS)
+                        v = load16(g.A + (long)m * g.lda, at, g.K);
+                    else if (at < g.K)
+                        v = *(const uint4 *)(tok + m * x.pitch + at);
+                }
+#pragma unroll
+                for (int r = 0; r < DOT_ROWS; r++) {
+                    int s = __dp4a((int)a[u][r].x, (int)v.x, acc[r][m]);
+                    s = __dp4a((int)a[u][r].y, (int)v.y, s);
+                    s = __dp4a((int)a[u][r].z, (int)v.z, s);
+                    acc[r][m] = __dp4a((int)a[u][r].w, (int)v.w, s);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < DOT_ROWS; r++)
+                a[u][r] = load16(w[r], at + U * step, g.K);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < DOT_ROWS; r++)
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            const int s = __reduce_add_sync(0xffffffffu, acc[r][m]);
+            if (lane == 0)
+                part[warp][r][m] = s;
+        }
+    __syncthreads();
+    if (!out)
+        return;
+    for (int m = m0; m < g.M; m += THREADS / channels) {
+        int s = 0;
+        for (int i = 0; i < split; i++)
+            s += part[c / DOT_ROWS * split + i][c % DOT_ROWS][m];
+        float v = act_any(scaled(s, scale[m], sb, bias), g.act, g.slope);
+        const long at = (long)m * g.ldc + c0 + c;
+        if (g.R)
+            v += ldf((const TC *)g.R + at);
+        stf((TC *)g.C + at, v);
+    }
 }
 
-constexpr int SKINNY_ROWS = 32;
+constexpr int DOT_TOKENS = 2;
+
+template <typename TC, typename TX>
+void few(cudaStream_t st, const I8Gemm &g, const Tokens &x, int sms)
+{
+    // The depth split as long as there are steps to share and fewer than two
+    // blocks per multiprocessor.
+    const bool dot = g.M <= DOT_TOKENS;
+    const int rows = dot ? DOT_ROWS : FEW_CH, step = dot ? DOT_STEP : FEW_STEP;
+    int split = 1;
+    while (split < FEW_WARPS && g.K > split * step &&
+           (long)g.N * split < 2L * sms * FEW_WARPS * rows)
+        split *= 2;
+    const unsigned grid = cdiv(g.N, FEW_WARPS / split * rows), T = 32 * FEW_WARPS;
+    const size_t smem = (size_t)x.pitch * g.M;
+    if (g.M <= 1 && dot)
+        launch_chained(i8_dot_k<1, TC, TX>, grid, T, smem, st, g, x, split);
+    else if (dot)
+        launch_chained(i8_dot_k<2, TC, TX>, grid, T, smem, st, g, x, split);
+    else if (g.M <= 8)
+        launch_chained(i8_few_k<1, TC, TX>, grid, T, smem, st, g, x, split);
+    else
+        launch_chained(i8_few_k<2, TC, TX>, grid, T, smem, st, g, x, split);
+}
+
+// Tokens that the streaming kernels take: up to two the dot products always;
+// up to 16 where the layer is no wider than the tensor cores' tiles fill the
+// device with (they take about 0.3 us per 128 bytes of depth at any width, these
+// 0.4 us per million weights up to 8 tokens and 0.6 up to 16: 8 tokens, 8192 x
+// 8192 32 against 21 us, 1024 x 1024 4.6 against 5.7).
+constexpr int FEW_ROWS = 16;
+bool streams(int M, int N)
+{
+    return M <= DOT_TOKENS || (M <= 8 && N <= 6144) || (M <= FEW_ROWS && N <= 4096);
+}
+
+// Rows that ops_linear_i8 quantises within the product: every block does it
+// again, so that it pays for few values only (16 x 1024 to 4096 channels 8.8 us
+// against 8.7 in two launches, 8 x 1024 6.4, one token 4.7 against 10).
+constexpr int FUSED_VALUES = 16384;
+bool fused(int rows, int in)
+{
+    return rows <= FEW_ROWS && (long)rows * in <= FUSED_VALUES;
+}
+
+void linear_fused(const struct ocl_backend *ocl, const I8Gemm &g, const View &X, int xtype)
+{
+    cudaStream_t st = stream_of(ocl);
+    const int sms = sms_of(ocl);
+    const Tokens x = {X.p, X.ld, token_pitch(g.K)};
+    if (xtype == OPS_BF16 && g.c_bf16)
+        few<__nv_bfloat16, __nv_bfloat16>(st, g, x, sms);
+    else if (xtype == OPS_BF16)
+        few<float, __nv_bfloat16>(st, g, x, sms);
+    else if (g.c_bf16)
+        few<__nv_bfloat16, float>(st, g, x, sms);
+    else
+        few<float, float>(st, g, x, sms);
+}
 
 void gemm_i8(const struct ocl_backend *ocl, const I8Gemm &g)
 {
     cudaStream_t st = stream_of(ocl);
-    if (g.M <= SKINNY_ROWS) {
+    if (streams(g.M, g.N)) {
+        const Tokens none = {nullptr, 0, 0};
         if (g.c_bf16)
-            skinny<__nv_bfloat16>(st, g);
+            few<__nv_bfloat16, void>(st, g, none, sms_of(ocl));
         else
-            skinny<float>(st, g);
+            few<float, void>(st, g, none, sms_of(ocl));
         return;
     }
     if (g.K > 0 && gemm_i8_tc(st, g, sms_of(ocl)))
@@ -541,7 +811,7 @@ static size_t work_scales(int rows) { return ((size_t)rows * 4 + 15) / 16 * 16; 
 
 extern "C" size_t ops_linear_i8_bytes(int rows, int in)
 {
-    return rows <= 0 || in < 0 ? 0 : work_scales(rows) + (size_t)rows * ops_i8_ld(in);
+    return rows <= 0 || in < 0 || fused(rows, in) ? 0 : work_scales(rows) + (size_t)rows * ops_i8_ld(in);
 }
 
 extern "C" void ops_linear_i8(struct ops *o, int rows, int in, int out, struct opnd X, int xtype,
@@ -576,8 +846,13 @@ extern "C" void ops_linear_i8(struct ops *o, int rows, int in, int out, struct o
     if (!dev.ok)
         return;
     cudaStream_t st = stream_of(o->ocl);
-    int8_t *q = (int8_t *)ws.p + work_scales(rows);
     Prof p(o->ocl, "linear_i8");
+    if (!bytes) {
+        linear_fused(o->ocl, g, x, xtype);
+        launch_ok("linear_i8");
+        return;
+    }
+    int8_t *q = (int8_t *)ws.p + work_scales(rows);
     quant_rows(st, x, xtype, q, ops_i8_ld(in), (float *)ws.p);
     g.A = q;
     g.lda = ops_i8_ld(in);

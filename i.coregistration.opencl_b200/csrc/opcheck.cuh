@@ -178,48 +178,38 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
 
 __device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
 
-// a b + c clamped to 0..1 (0 for NaN).
-__device__ __forceinline__ float fma_sat(float a, float b, float c)
+// 2^x, to 2 units of the last place.
+__device__ __forceinline__ float exp2_fast(float x)
 {
     float d;
-    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
     return d;
 }
 
-// Exact GELU, x Phi(x), of two values. Phi(x) = 0.5 + x Q(min(x^2, X^2)),
-// clamped to 0..1, where Q is the polynomial in s = 2 x^2 / X^2 - 1 with the
-// least largest error of x Q over |x| <= X (fitted here in 64 bits). FINE:
-// degree 14, X = 5.4, and Phi off by at most 1.3e-7 in float32 arithmetic, as 0.5
-// (1 + erff(x / sqrt 2)) is by 0.6e-7; otherwise degree 12, X = 5.2, 4.3e-7,
-// which is for results that are rounded to bfloat16 (2^-8). At X, x Q passes
-// 0.5, so that larger |x| give exactly x or 0. In packed multiply-adds but for
-// four operations of a pair: about half the issue slots of CUDA's erff in
-// the same formula, which bounded the epilogue of the 8-bit product.
-template <bool FINE>
+// Exact GELU, x Phi(x), of two values, as x / (1 + 2^(x Q(x^2))): log2(Phi(-x) /
+// Phi(x)) / x is a smooth even function, and Q the polynomial of degree 6 in
+// min(x^2, 25) that brings Phi nearest to it (fitted here in 64 bits,
+// weighted by the derivative Phi (1 - Phi) x). In float32 Phi is off by at
+// most 1.0e-7 (0.5 (1 + erff(x / sqrt 2)) by 0.6e-7) and by 5e-5 of itself down
+// to x = -3, where the other form has lost that too; 1 and 0 follow far out.
+// Nine multiply-adds, packed in pairs, and two steps of the special function
+// unit: half the work of erff's polynomials, which bounded the 8-bit
+// product's epilogue.
 __device__ __forceinline__ float2 gelu2(float2 x)
 {
-    constexpr int D = FINE ? 14 : 12;
-    constexpr float X = FINE ? 5.4f : 5.2f;
-    constexpr float Q14[15] = {
-        0.13092811405658722f,    -0.06532805413007736f,  0.04849959164857864f,
-        -0.03920681402087212f,   0.03211659565567970f,   -0.02574645727872848f,
-        0.01964514516294003f,    -0.01396332029253245f,  0.00965119525790214f,
-        -0.006715338211506605f,  0.003658922854810953f,  -0.0011864101979881525f,
-        0.0008749334374442696f,  -0.0010283688316121697f, 0.00039285887032747269f};
-    constexpr float Q12[13] = {
-        0.13594993948936462f,  -0.06774269789457321f,  0.05002840608358383f,
-        -0.03995957598090172f, 0.03193814679980278f,   -0.024464763700962067f,
-        0.01820363663136959f,  -0.013464033603668213f, 0.008026459254324436f,
-        -0.003071868559345603f, 0.002321982756257057f, -0.0026904314290732145f,
-        0.0010786805069074035f};
+    constexpr float Q[7] = {-2.302206516265869f,      -0.10484472662210464f,
+                            0.00010274611122440547f,  0.000156551250256598f,
+                            -1.098385200748453e-05f,  3.5264929465483874e-07f,
+                            -4.4573145174808815e-09f};
     float2 u = fma2(x, x, pair(0.0f));
-    u = make_float2(fminf(u.x, X * X), fminf(u.y, X * X));
-    const float2 s = fma2(u, pair(2.0f / (X * X)), pair(-1.0f));
-    float2 q = pair(FINE ? Q14[D] : Q12[D <= 12 ? D : 0]);
+    u = make_float2(fminf(u.x, 25.0f), fminf(u.y, 25.0f));
+    float2 q = pair(Q[6]);
 #pragma unroll
-    for (int i = D - 1; i >= 0; i--)
-        q = fma2(q, s, pair(FINE ? Q14[i] : Q12[i <= 12 ? i : 0]));
-    return fma2(x, make_float2(fma_sat(x.x, q.x, 0.5f), fma_sat(x.y, q.y, 0.5f)), pair(0.0f));
+    for (int i = 5; i >= 0; i--)
+        q = fma2(q, u, pair(Q[i]));
+    q = fma2(x, q, pair(0.0f));
+    return make_float2(__fdividef(x.x, 1.0f + exp2_fast(q.x)),
+                       __fdividef(x.y, 1.0f + exp2_fast(q.y)));
 }
 
 // The larger value, or NaN where one is (fmaxf would drop it).
@@ -237,13 +227,13 @@ __device__ __forceinline__ float times_sigmoid(float v, float t)
     return __fdividef(v, 1.0f + __expf(-t));
 }
 
-// The activation of two values, FINE as in gelu2. GELU_TANH is v sigmoid(2 y)
-// with y the argument of its tanh.
-template <int ACT, bool FINE>
+// The activation of two values. GELU_TANH is v sigmoid(2 y) with y the
+// argument of its tanh.
+template <int ACT>
 __device__ __forceinline__ float2 act2(float2 v, float slope)
 {
     if (ACT == ACT_GELU)
-        return gelu2<FINE>(v);
+        return gelu2(v);
     if (ACT == ACT_RELU)
         return make_float2(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f));
     if (ACT == ACT_LEAKY)
@@ -262,7 +252,7 @@ __device__ __forceinline__ float2 act2(float2 v, float slope)
 template <int ACT>
 __device__ __forceinline__ float act1(float v, float slope)
 {
-    return act2<ACT, true>(make_float2(v, 0.0f), slope).x;
+    return act2<ACT>(make_float2(v, 0.0f), slope).x;
 }
 
 // The same with the activation known at run time only.

@@ -166,14 +166,6 @@ __device__ __forceinline__ void stage_row(unsigned char *blk, int l, int h, cons
     }
 }
 
-// First k-block of tile t: tiles that share rows of A or of B begin their
-// depth at different blocks, so that the CTAs running at one time do not all
-// ask L2 for the same lines (the sums are integers: no order changes them).
-__device__ __forceinline__ int first_block(int t, int tiles_m, int nk)
-{
-    return (int)(((unsigned)(t % tiles_m) * 5u + (unsigned)(t / tiles_m) * 3u) % (unsigned)nk);
-}
-
 // One epilogue warp's part of a tile: TMEM lanes 32 q .. (rows of the tile from
 // m0 on) and the blocks part, part + 4, ... of columns (from n0 on) of the
 // accumulator acc, which is complete when `full` turns `parity`. Returns false
@@ -226,7 +218,7 @@ __device__ __forceinline__ bool tile_out(const Params &p, const CUtensorMap *tma
                 const float2 y = fma2(make_float2(__int2float_rn(__float_as_int(v[j])),
                                                   __int2float_rn(__float_as_int(v[j + 1]))),
                                       pair(sa), pair(0.0f));
-                const float2 x = act2<ACT, sizeof(TC) == 4>(
+                const float2 x = act2<ACT>(
                     fma2(y, make_float2(sb[j], sb[j + 1]),
                          g.bias ? make_float2(bias[j], bias[j + 1]) : pair(0.0f)),
                     g.slope);
@@ -302,9 +294,7 @@ tc_i8_k(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUten
             bool ok = true;
             for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
                 const int m0 = (t % tiles_m) * BM, n0 = (t / tiles_m) * BN;
-                const int off = first_block(t, tiles_m, nk);
-                for (int k = 0; k < nk; k++, it++) {
-                    const int kb = k + off < nk ? k + off : k + off - nk;
+                for (int kb = 0; kb < nk; kb++, it++) {
                     const int st = it % ST;
                     if (it >= ST && !mbar_wait(&s.empty[st], ((it / ST) - 1) & 1, 61)) {
                         ok = false;

@@ -143,6 +143,11 @@ GEMM = [
     (700, 24, 48, 0, 0, 0),
     (1000, 777, 333, 0, 0, 7),
     (513, 16, 9000, 0, 0, 0),
+    (2, 7000, 700, 0, 0, 0),
+    (3, 6145, 530, 0, 0, 0),
+    (8, 6144, 96, 0, 0, 0),
+    (9, 4096, 200, 16, 1, 1),
+    (16, 4100, 144, 0, 0, 0),
 ]
 
 
@@ -211,7 +216,14 @@ LINEAR = [
     (1, 1024, 4096, 0, 0),
     (2, 1000, 50, 0, 0),
     (5, 37, 129, 3, 2),
+    (1, 16384, 33, 0, 0),
+    (1, 16385, 33, 0, 0),
+    (2, 515, 40, 1, 0),
+    (3, 4099, 70, 0, 0),
+    (4, 4096, 130, 0, 1),
     (8, 4096, 256, 0, 0),
+    (9, 1500, 5000, 0, 4),
+    (16, 1024, 16, 0, 0),
     (16, 512, 512, 8, 8),
     (17, 5000, 64, 0, 0),
     (32, 2048, 100, 0, 0),
