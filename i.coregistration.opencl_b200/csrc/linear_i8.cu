@@ -23,7 +23,8 @@ namespace {
 // exact in one fused multiply-add: x and s are multiples of the smaller of
 // their last places, and the difference is below s (in units of that place
 // below 2^24). So |x - q s| against s / 2 decides, without a division, and
-// the seldom values that it moves take a branch.
+// pieces with a value that it may move take a branch (1 in 10 of random
+// tokens; of bfloat16 rows whose largest value is 127 2^n, half are ties).
 struct RowScale {
     float s, inv, half;
     __device__ explicit RowScale(uint32_t amax)
@@ -37,6 +38,9 @@ struct RowScale {
                 inv = __fdiv_rn(1.0f, s);
                 half = 0.5f * s;
             }
+            else if (amax == 0) {
+                half = 1.0f; // every value of a row of zeros is sure to be 0
+            }
         }
     }
     // The quantised value as the low byte of the result; sure: whether it is.
@@ -47,12 +51,25 @@ struct RowScale {
         sure = sure && fabsf(d) < half;
         return __float_as_uint(big);
     }
-    // Any value of any row: next to a tie, or of a scale that is not a normal
-    // positive number.
-    __device__ __noinline__ uint32_t slow(float x) const
+    // The value for a guess g of x that was not sure, in a row with inv > 0.
+    __device__ __forceinline__ uint32_t settle(uint32_t g, float x) const
+    {
+        const float d = fmaf(12582912.0f - __uint_as_float(g), s, x), e = fabsf(d);
+        if (e > half || (e == half && (g & 1)))
+            g += d > 0.0f ? 1u : ~0u;
+        return g;
+    }
+    __device__ __forceinline__ uint32_t of(float x) const
+    {
+        bool sure = true;
+        const uint32_t q = guess(x, sure);
+        return sure ? q : quotient(x, s);
+    }
+    // Any value of any row.
+    static __device__ __noinline__ uint32_t quotient(float x, float s)
     {
         if (!(s > 0.0f))
-            return 0; // a row of zeros, or with an infinity or NaN
+            return 0; // a scale of 0, or a row with an infinity or NaN
         // Small scales into the normal range by an exact power of two.
         const float k = s < 0x1p-90f ? 0x1p+90f : 1.0f, u = s * k;
         x *= k;
@@ -61,12 +78,6 @@ struct RowScale {
         if (e > u || (e == u && ((int)q & 1)))
             q += copysignf(1.0f, d);
         return (uint32_t)(int)fminf(fmaxf(q, -127.0f), 127.0f);
-    }
-    __device__ __forceinline__ uint32_t of(float x) const
-    {
-        bool sure = true;
-        const uint32_t q = guess(x, sure);
-        return sure ? q : slow(x);
     }
 };
 
@@ -89,13 +100,19 @@ struct Piece {
         const uint32_t x = i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
         return __uint_as_float(sizeof(T) == 4 ? x : e % 2 ? x & 0xffff0000u : x << 16);
     }
+    // Bits of the largest magnitude, as a float's.
     __device__ __forceinline__ uint32_t top() const
     {
-        uint32_t m = 0;
-#pragma unroll
-        for (int e = 0; e < V; e++)
-            m = max(m, magnitude(at(e)));
-        return m;
+        if constexpr (sizeof(T) == 4) {
+            return max(max(magnitude(at(0)), magnitude(at(1))),
+                       max(magnitude(at(2)), magnitude(at(3))));
+        }
+        else {
+            // Two at a time: bfloat16 orders as float does.
+            const uint32_t k = 0x7fff7fffu;
+            const uint32_t m = __vmaxu2(__vmaxu2(w.x & k, w.y & k), __vmaxu2(w.z & k, w.w & k));
+            return max(m << 16, m & 0xffff0000u);
+        }
     }
     __device__ __forceinline__ void store(int8_t *q, const RowScale &s) const
     {
@@ -105,15 +122,33 @@ struct Piece {
         for (int e = 0; e < V; e++)
             v[e] = s.guess(at(e), sure);
         if (!sure) {
+            if (!(s.inv > 0.0f)) {
+                store_slow(w, q, s.s);
+                return;
+            }
 #pragma unroll
             for (int e = 0; e < V; e++)
-                v[e] = s.slow(at(e));
+                v[e] = s.settle(v[e], at(e));
         }
-        if constexpr (V == 4) {
+        if constexpr (V == 4)
             *(uint32_t *)q = pack4(v[0], v[1], v[2], v[3]);
-        }
-        else {
+        else
             *(uint2 *)q = make_uint2(pack4(v[0], v[1], v[2], v[3]), pack4(v[4], v[5], v[6], v[7]));
+    }
+    // (Rows of denormal scales, infinities or NaN.)
+    static __device__ __noinline__ void store_slow(uint4 w, int8_t *q, float s)
+    {
+        Piece<T, V> p;
+        p.w = w;
+#pragma unroll 1
+        for (int e = 0; e < V; e++) {
+            const float x = p.at(0);
+            q[e] = (int8_t)RowScale::quotient(x, s);
+            // The next value to the front.
+            if (sizeof(T) == 4 || e % 2)
+                p.w = make_uint4(p.w.y, p.w.z, p.w.w, 0);
+            else
+                p.w.x >>= 16;
         }
     }
 };
