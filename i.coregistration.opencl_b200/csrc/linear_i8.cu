@@ -278,43 +278,21 @@ __device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias)
     return fmaf(__int2float_rn(acc) * sa, sb, bias);
 }
 
-// 64 x 64 output tiles, 4 x 4 sums per thread, 64 bytes of depth staged at a
-// time; four products per __dp4a.
+// Products of depth 0: act(bias) + R.
 template <typename TC>
 __global__ void __launch_bounds__(256)
-i8_tile_k(const I8Gemm g)
+i8_empty_k(const I8Gemm g)
 {
-    __shared__ uint32_t a[64][17], b[64][17];
-    const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    int acc[4][4] = {};
-    for (int k0 = 0; k0 < g.K; k0 += 64) {
-        for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-            const int r = i / 64, k = i % 64;
-            const bool in = k0 + k < g.K;
-            ((int8_t *)a[r])[k] =
-                in && m0 + r < g.M ? g.A[(long)(m0 + r) * g.lda + k0 + k] : (int8_t)0;
-            ((int8_t *)b[r])[k] =
-                in && n0 + r < g.N ? g.B[(long)(n0 + r) * g.ldb + k0 + k] : (int8_t)0;
-        }
-        __syncthreads();
-        for (int k = 0; k < 16; k++)
-            for (int i = 0; i < 4; i++)
-                for (int j = 0; j < 4; j++)
-                    acc[i][j] = __dp4a((int)a[ty + 16 * i][k], (int)b[tx + 16 * j][k], acc[i][j]);
-        __syncthreads();
+    after_previous();
+    const long n = (long)g.M * g.N;
+    for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long)gridDim.x * 256) {
+        const long m = e / g.N, c = e - m * g.N, at = m * g.ldc + c;
+        float v = act_any(scaled(0, g.sa ? g.sa[m] : 0.0f, g.sb[c], g.bias ? g.bias[c] : 0.0f),
+                          g.act, g.slope);
+        if (g.R)
+            v += ldf((const TC *)g.R + at);
+        stf((TC *)g.C + at, v);
     }
-    for (int i = 0; i < 4; i++)
-        for (int j = 0; j < 4; j++) {
-            const int r = m0 + ty + 16 * i, c = n0 + tx + 16 * j;
-            if (r >= g.M || c >= g.N)
-                continue;
-            float v = scaled(acc[i][j], g.sa[r], g.sb[c], g.bias ? g.bias[c] : 0.0f);
-            v = act_any(v, g.act, g.slope);
-            if (g.R)
-                v += ldf((const TC *)g.R + (long)r * g.ldc + c);
-            stf((TC *)g.C + (long)r * g.ldc + c, v);
-        }
 }
 
 // Few tokens: the weights stream once from memory. A warp takes 16 of their
@@ -697,16 +675,26 @@ void gemm_i8(const struct ocl_backend *ocl, const I8Gemm &g)
             few<float, void>(st, g, none, sms_of(ocl));
         return;
     }
-    if (g.K > 0 && gemm_i8_tc(st, g, sms_of(ocl)))
+    if (g.K == 0) {
+        const unsigned grid = 8 * sms_of(ocl);
+        if (g.c_bf16)
+            launch_chained(i8_empty_k<__nv_bfloat16>, grid, 256, 0, st, g);
+        else
+            launch_chained(i8_empty_k<float>, grid, 256, 0, st, g);
         return;
-    const dim3 grid(cdiv(g.N, 64), cdiv(g.M, 64));
-    if (g.c_bf16)
-        i8_tile_k<__nv_bfloat16><<<grid, 256, 0, st>>>(g);
-    else
-        i8_tile_k<float><<<grid, 256, 0, st>>>(g);
+    }
+    if (!gemm_i8_tc(st, g, sms_of(ocl)))
+        fail("8-bit product of %d x %d x %d: the tensor cores refused the operands", g.M, g.N, g.K);
 }
 
+}  // namespace
+
+namespace {
+
 // -------------------------------------------------------------- arguments
+
+// Rows and columns whose tile indexes stay within 31 bits.
+constexpr int I8_MAX_ROWS = 0x7ffffe00;
 
 // An int8 operand of the product: rows 16-byte aligned.
 bool i8_view(View *v, const char *fn, const char *what, const struct opnd &m, long rows, long K)
@@ -729,7 +717,7 @@ bool product_args(const char *fn, I8Gemm *g, int M, int N, int K, const struct o
                   float slope, View *out, View in[4], int *nin)
 {
     View r;
-    if (M < 0 || N < 0 || K < 0 || K > OPS_I8_MAX_K) {
+    if (M < 0 || N < 0 || K < 0 || K > OPS_I8_MAX_K || M > I8_MAX_ROWS || N > I8_MAX_ROWS) {
         fail("%s: %d x %d x %d (depth 0..%d)", fn, M, N, K, OPS_I8_MAX_K);
         return false;
     }
@@ -765,7 +753,7 @@ bool product_args(const char *fn, I8Gemm *g, int M, int N, int K, const struct o
     g->M = M;
     g->N = N;
     g->K = K;
-    g->ldb = B.ld;
+    g->ldb = N > 1 ? B.ld : ops_i8_ld(K); // (a single row's pitch may be anything)
     g->C = out->p;
     g->ldc = C.ld;
     g->c_bf16 = ctype == OPS_BF16;
@@ -800,6 +788,10 @@ extern "C" void ops_quant_i8(struct ops *o, long rows, int C, struct opnd X, int
         !view_of(&out[0], fn, "Q", Q.buf, Q.off, Q.ld, rows, C, 1) ||
         !view_of(&out[1], fn, "S", S, soff, 1, rows, 1, 4) || !count_ok(rows, "rows of int8"))
         return;
+    if (C > 0x40000000) {
+        fail("%s: rows of %d (at most 2^30)", fn, C);
+        return;
+    }
     if (!apart(fn, out[0], &in, 1) || !apart(fn, out[1], &in, 1) || !apart(fn, out[0], out + 1, 1))
         return;
     if (rows == 0 || C == 0)
@@ -831,7 +823,7 @@ extern "C" void ops_gemm_i8(struct ops *o, int M, int N, int K, struct opnd A, c
     if (M == 0 || N == 0)
         return;
     g.A = (const int8_t *)in[n].p;
-    g.lda = A.ld;
+    g.lda = M > 1 ? A.ld : ops_i8_ld(K);
     g.sa = (const float *)in[n + 1].p;
     OnDevice dev(o->ocl);
     if (!dev.ok)

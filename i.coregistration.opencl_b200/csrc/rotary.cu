@@ -310,7 +310,7 @@ extern "C" void ops_rotary(struct ops *o, const struct ops_rotary *r, long rows,
         fail("%s: no frequencies (ops_rotary_plan)", fn);
         return;
     }
-    if (nh < 0 || d < r->rot || (long)nh * d > 0x7fffffffL) {
+    if (nh < 0 || d < r->rot || (long)nh * d > 0x40000000L) {
         fail("%s: %d heads of %d columns, %d rotated", fn, nh, d, r->rot);
         return;
     }

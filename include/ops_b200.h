@@ -115,7 +115,8 @@ size_t ops_gemm_noalloc_max_bytes(void);
  * a multiple of 16. */
 int ops_i8_ld(int K);
 
-/* Rows of X (rows x C, type xtype) to 8-bit integers with one scale each:
+/* Rows of X (rows x C, C at most 2^30, type xtype) to 8-bit integers with
+ * one scale each:
  *   s = max |x| / 127 (float32, rounded to nearest), q = x / s
  * rounded to the nearest integer (ties to even; decided on the exact
  * quotient) within -127..127. Q holds bytes (Q.ld in bytes), S float32
@@ -183,8 +184,8 @@ struct ops_rotary {
 void ops_rotary_plan(struct ops_rotary *r, int rot, int axes, int interleaved, double base,
                      int scaling, double factor, long length);
 
-/* Rotary positions of rows x nh heads of d columns (a token's heads beside
- * each other: the queries, or queries and keys, of a qkv buffer): Y = X
+/* Rotary positions of rows x nh heads of d columns (at most 2^30 in a row; a
+ * token's heads beside each other: the queries, or queries and keys, of a qkv buffer): Y = X
  * with each pair (a, b) of a head's first r->rot columns replaced by
  * mscale (a cos t - b sin t, a sin t + b cos t), t = w_f p, and the other
  * columns as they were. p is pos0 plus the token's entry of pos (int32,

@@ -142,6 +142,70 @@ def test_block_captured_and_replayed():
     dev.close()
 
 
+FIRST_CALL = """
+import sys
+sys.path[:0] = {path!r}
+import ctypes as C
+import numpy as np
+import coreg
+from oracle import ops_b200_ref as ref
+rt = C.CDLL("libcudart.so.12")
+dev = coreg.Device(0)
+lib, o, m = dev.lib, dev.ops_p, coreg.Opnd
+rng = np.random.default_rng(0)
+# Every kind of launch: a whole-device team, a cluster team, tensor cores,
+# streamed weights, the quantiser, the rotation.
+maps = [(2, 260000, 64), (1, 500, 64)]
+xs = [rng.standard_normal(s).astype(np.float32) for s in maps]
+X = [dev.upload(x) for x in xs]
+Y = [dev.zeros(x.size) for x in xs]
+work = [dev.alloc(lib.ops_groupnorm_cl_bytes(*s, 8)) for s in maps]
+M, K = 200, 128
+t = rng.standard_normal((M, K)).astype(np.float32)
+qw, sw = ref.quant_i8(rng.standard_normal((K, K)))
+T, Q, S, QW, SW, Z, R = (dev.upload(t), dev.alloc(M * K), dev.zeros(M), dev.upload(qw),
+                         dev.upload(sw), dev.zeros(M * K), dev.zeros(M * K))
+P = coreg.Rotary()
+lib.ops_rotary_plan(P, 64, 1, 1, 100.0, 0, 1.0, 1)
+st, graph, exe = C.c_void_p(dev.ocl.queue), C.c_void_p(), C.c_void_p()
+assert rt.cudaStreamBeginCapture(st, 1) == 0
+for x, y, w, s in zip(X, Y, work, maps):
+    lib.ops_groupnorm_cl(o, *s, 8, m(x.handle, 0, 64, s[1] * 64, 0), 0,
+                         m(y.handle, 0, 64, s[1] * 64, 0), 0, None, None, 1e-5, 0, 0.0, w.handle)
+lib.ops_quant_i8(o, M, K, m(T.handle, 0, K, 0, 0), 0, m(Q.handle, 0, K, 0, 0), S.handle, 0)
+for rows in (M, 5, 1):
+    lib.ops_gemm_i8(o, rows, K, K, m(Q.handle, 0, K, 0, 0), S.handle, m(QW.handle, 0, K, 0, 0),
+                    SW.handle, None, m(Z.handle, 0, K, 0, 0), 0, None, 0, 0, 0.0)
+lib.ops_rotary(o, P, M, 2, 64, m(Z.handle, 0, K, 0, 0), m(R.handle, 0, K, 0, 0), 0, None, 0)
+coreg.check(lib)
+assert rt.cudaStreamEndCapture(st, C.byref(graph)) == 0
+assert rt.cudaGraphInstantiate(C.byref(exe), graph, 0) == 0
+for turn in range(3):
+    assert rt.cudaGraphLaunch(exe, st) == 0
+for x, y in zip(xs, Y):
+    want = ref.groupnorm(x, 8)
+    assert np.abs(y.read().reshape(x.shape) - want).max() < 1e-4
+z, _ = ref.gemm_i8(*ref.quant_i8(t), qw, sw)
+w, _ = ref.frequencies(64, 1, 100.0)
+want = ref.rotary(z, np.arange(M)[:, None], 2, 64, 64, 1, 1, w)
+assert np.abs(R.read().reshape(M, K) - want).max() < 1e-4 * np.abs(want).max()
+print("captured first")
+"""
+
+
+@pytest.mark.gpu
+def test_first_calls_of_a_process_captured():
+    """A process whose first call of every entry point is the captured one."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    root = Path(__file__).resolve().parents[1]
+    code = FIRST_CALL.format(path=[str(root), str(root / "i.coregistration.opencl_b200")])
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stderr[-2000:]
+
+
 @pytest.mark.gpu
 def test_two_backends_at_once():
     """Two blocks with their own buffers on two streams, many runs under way

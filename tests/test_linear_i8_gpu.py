@@ -148,6 +148,7 @@ GEMM = [
     (8, 6144, 96, 0, 0, 0),
     (9, 4096, 200, 16, 1, 1),
     (16, 4100, 144, 0, 0, 0),
+    (300, 1, 200, 0, 0, 0),
 ]
 
 
@@ -208,6 +209,23 @@ def test_gemm_largest_sums(dev, M):
     dev.lib.ops_gemm_i8(dev.ops_p, M, N, 0, A.opnd, S.handle, B.opnd, S.handle, bias.handle,
                         C.opnd, F32, None, 0, coreg.ACT_RELU, 0.0)
     assert (C.read() == np.maximum(np.arange(N) - 7, 0)).all()
+
+
+@pytest.mark.gpu
+def test_gemm_single_rows_of_any_pitch(dev):
+    """A pitch that a single row of weights or tokens does not have is not used."""
+    K = 100
+    rng = np.random.default_rng(1)
+    for M, N in ((40, 1), (1, 40)):
+        a, sa, b, sb, _ = operands(rng, M, N, K)
+        A, B, SA, SB = i8_rows(dev, a), i8_rows(dev, b), dev.upload(sa), dev.upload(sb)
+        C = Rows(dev, M, N, F32)
+        oa, ob = A.opnd, B.opnd
+        (ob if N == 1 else oa).ld = -7
+        dev.lib.ops_gemm_i8(dev.ops_p, M, N, K, oa, SA.handle, ob, SB.handle, None, C.opnd, F32,
+                            None, 0, 0, 0.0)
+        want, mag = ref.gemm_i8(a, sa, b, sb)
+        close(C.read(), want, tolerance(want, mag, None, F32))
 
 
 LINEAR = [

@@ -72,6 +72,7 @@ def test_quant_refusals(h):
     h.refuses("passes its buffer", f, 4, 8, M(X, 8, 2 ** 62), F32, M(Q, 16), S, 0)
     h.refuses("passes its buffer", f, 2 ** 62, 8, M(X, 2 ** 31 - 1), F32, M(Q, 16), S, 0)
     h.refuses("not aligned", f, 4, 8, M(h.buf(1024, 2), 8), F32, M(Q, 16), S, 0)
+    h.refuses("rows of 1073741825", f, 0, 2 ** 30 + 1, M(X, 8), F32, M(Q, 8), S, 0)
     h.refuses("overlaps", f, 4, 8, M(X, 8), F32, M(X, 8, 100), S, 0)
     h.refuses("overlaps", f, 4, 8, M(X, 8), F32, M(Q, 8), X, 3)
     h.refuses("overlaps", f, 4, 8, M(X, 8), F32, M(Q, 8), Q, 0)
@@ -92,6 +93,8 @@ def test_gemm_refusals(h):
     h.refuses("4 x -8", f, *args(n=-8))
     h.refuses("4 x 8 x -1", f, *args(k=-1))
     h.refuses("depth 0..131071", f, *args(k=131072))
+    h.refuses("2147483647 x 8", f, *args(m=2 ** 31 - 1))
+    h.refuses("4 x 2147483647", f, *args(n=2 ** 31 - 1))
     h.refuses("element type 7", f, *args(t=7))
     h.refuses("activation 6", f, *args(act=6))
     h.refuses("activation -1", f, *args(act=-1))
@@ -163,6 +166,7 @@ def test_rotary_refusals(h):
     h.refuses("8 rotated", f, *args(d=7))
     h.refuses("-2 heads", f, *args(nh=-2))
     h.refuses("heads", f, *args(nh=2 ** 30))
+    h.refuses("heads", f, *args(nh=2 ** 27, d=16))
     h.refuses("element type 5", f, *args(t=5))
     h.refuses("two axes need positions", f, *args(plan=two, p=None))
     h.refuses("X is NULL", f, *args(x=M(None, 20)))
