@@ -186,15 +186,33 @@ __device__ __forceinline__ float exp2_fast(float x)
     return d;
 }
 
+__device__ __forceinline__ float rcp_fast(float x)
+{
+    float d;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
+    return d;
+}
+
+// x / (1 + 2^z) of two values, by one reciprocal for both: the special function
+// unit takes 8 cycles an instruction and warp, and bounds these. Exponents
+// are cut off at 60, where the quotient is below 1e-18 of x, so that the
+// product of the two divisors stays in range. Relative error below 4e-7 for
+// exact z.
+__device__ __forceinline__ float2 over_one_plus_exp2(float2 x, float2 z)
+{
+    const float a = 1.0f + exp2_fast(fminf(z.x, 60.0f)), b = 1.0f + exp2_fast(fminf(z.y, 60.0f));
+    const float r = rcp_fast(a * b);
+    return make_float2(x.x * (b * r), x.y * (a * r));
+}
+
 // Exact GELU, x Phi(x), of two values, as x / (1 + 2^(x Q(x^2))): log2(Phi(-x) /
 // Phi(x)) / x is a smooth even function, and Q the polynomial of degree 6 in
 // min(x^2, 25) that brings Phi nearest to it (fitted here in 64 bits,
 // weighted by the derivative Phi (1 - Phi) x). In float32 Phi is off by at
-// most 1.0e-7 (0.5 (1 + erff(x / sqrt 2)) by 0.6e-7) and by 5e-5 of itself down
+// most 1.5e-7 (0.5 (1 + erff(x / sqrt 2)) by 0.6e-7) and by 5e-5 of itself down
 // to x = -3, where the other form has lost that too; 1 and 0 follow far out.
-// Nine multiply-adds, packed in pairs, and two steps of the special function
-// unit: half the work of erff's polynomials, which bounded the 8-bit
-// product's epilogue.
+// Half the work of erff's polynomials, which bounded the 8-bit product's
+// epilogue.
 __device__ __forceinline__ float2 gelu2(float2 x)
 {
     constexpr float Q[7] = {-2.302206516265869f,      -0.10484472662210464f,
@@ -207,9 +225,7 @@ __device__ __forceinline__ float2 gelu2(float2 x)
 #pragma unroll
     for (int i = 5; i >= 0; i--)
         q = fma2(q, u, pair(Q[i]));
-    q = fma2(x, q, pair(0.0f));
-    return make_float2(__fdividef(x.x, 1.0f + exp2_fast(q.x)),
-                       __fdividef(x.y, 1.0f + exp2_fast(q.y)));
+    return over_one_plus_exp2(x, fma2(x, q, pair(0.0f)));
 }
 
 // The larger value, or NaN where one is (fmaxf would drop it).
@@ -220,15 +236,8 @@ __device__ __forceinline__ float max_nan(float a, float b)
     return d;
 }
 
-// v / (1 + e^-t) by the fast exponential and division: relative error below
-// 4e-7 (1 + |t|). Where e^-t overflows the quotient is 0, the limit.
-__device__ __forceinline__ float times_sigmoid(float v, float t)
-{
-    return __fdividef(v, 1.0f + __expf(-t));
-}
-
-// The activation of two values. GELU_TANH is v sigmoid(2 y) with y the
-// argument of its tanh.
+// The activation of two values. GELU_TANH is v sigmoid(2 y) with y the argument
+// of its tanh, SiLU v sigmoid(v).
 template <int ACT>
 __device__ __forceinline__ float2 act2(float2 v, float slope)
 {
@@ -239,13 +248,13 @@ __device__ __forceinline__ float2 act2(float2 v, float slope)
     if (ACT == ACT_LEAKY)
         return make_float2(v.x >= 0.0f ? v.x : slope * v.x, v.y >= 0.0f ? v.y : slope * v.y);
     if (ACT == ACT_GELU_TANH) {
-        constexpr float k = 1.5957691216057308f; // 2 sqrt(2 / pi)
-        return make_float2(
-            times_sigmoid(v.x, k * v.x * fmaf(0.044715f * v.x, v.x, 1.0f)),
-            times_sigmoid(v.y, k * v.y * fmaf(0.044715f * v.y, v.y, 1.0f)));
+        // 2^(-2 y / ln 2): -2 sqrt(2 / pi) / ln 2 and 0.044715 of that.
+        const float2 u = fma2(v, v, pair(0.0f));
+        const float2 q = fma2(u, pair(-0.1029432395800235f), pair(-2.302208198144325f));
+        return over_one_plus_exp2(v, fma2(v, q, pair(0.0f)));
     }
     if (ACT == ACT_SILU)
-        return make_float2(times_sigmoid(v.x, v.x), times_sigmoid(v.y, v.y));
+        return over_one_plus_exp2(v, fma2(v, pair(-1.4426950408889634f), pair(0.0f)));
     return v;
 }
 

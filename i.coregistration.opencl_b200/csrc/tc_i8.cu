@@ -18,6 +18,8 @@
 // Bytes of a row behind K, rows behind M and N: outside the tensor maps,
 // which read them as zeros. Every mbarrier wait is bounded (tc_common.cuh).
 
+#include <type_traits>
+
 #include "linear_i8.cuh"
 #include "tc_common.cuh"
 
@@ -30,7 +32,9 @@ constexpr int BM = 128, BK = 128; // BK in bytes
 // of their chain (scales, TMEM, activation, staging) bound the kernel, 10.8
 // thousand cycles a 128 x 256 tile with GELU against 4.3 of its products.
 constexpr int EPI_WARPS = 16, NTHREADS = 64 + 32 * EPI_WARPS;
-// Bytes of an output block's row: 16 columns of float, 32 of bfloat16.
+// Bytes of an output block's row: 16 columns of float, 32 of bfloat16. (Rows of
+// 128 bytes cost a stage of the ring, which costs more: CTA pairs with four
+// stages and such rows 154 us against 145 with five.)
 constexpr int ROW = 64;
 
 struct Params {
@@ -83,7 +87,7 @@ __device__ __forceinline__ void load_cols(float v[16], const float *p, int col, 
     if (whole) {
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
-            const float4 x = __ldg((const float4 *)(p + j));
+            const float4 x = *(const float4 *)(p + j);
             v[j] = x.x;
             v[j + 1] = x.y;
             v[j + 2] = x.z;
@@ -93,7 +97,7 @@ __device__ __forceinline__ void load_cols(float v[16], const float *p, int col, 
     }
 #pragma unroll
     for (int j = 0; j < 16; j++)
-        v[j] = col + j < n ? __ldg(p + j) : 0.0f;
+        v[j] = col + j < n ? p[j] : 0.0f;
 }
 
 // The 16 values of a residual row from R on, zero behind n; whole: they exist
@@ -148,7 +152,8 @@ __device__ __forceinline__ void stage_row(unsigned char *blk, int l, int, const 
 {
 #pragma unroll
     for (int c = 0; c < 4; c++)
-        *(float4 *)chunk(blk, l, c) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+        *(float4 *)chunk(blk, l, c) =
+            make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
 }
 
 __device__ __forceinline__ void stage_row(unsigned char *blk, int l, int h, const float v[16],
@@ -168,13 +173,15 @@ __device__ __forceinline__ void stage_row(unsigned char *blk, int l, int h, cons
 
 // One epilogue warp's part of a tile: TMEM lanes 32 q .. (rows of the tile from
 // m0 on) and the blocks part, part + 4, ... of columns (from n0 on) of the
-// accumulator acc, which is complete when `full` turns `parity`. Returns false
-// when that wait ran out; else the warp's reads of the accumulator are done.
-template <int BN, int ACT, typename TC>
+// accumulator acc, which is complete when `full` turns `parity`. SHARED: the
+// scales and the bias of the tile's columns are in shared memory at cols and
+// cols + BN. Returns false when that wait ran out; else the warp's reads of
+// the accumulator are done.
+template <int BN, bool SHARED, int ACT, typename TC>
 __device__ __forceinline__ bool tile_out(const Params &p, const CUtensorMap *tma_c,
                                          unsigned char *cst, uint32_t acc, uint64_t *full,
                                          uint32_t parity, int m0, int n0, int q, int part,
-                                         int lane)
+                                         int lane, const float *cols)
 {
     constexpr int COLS = ROW / (int)sizeof(TC); // of a block
     const I8Gemm &g = p.g;
@@ -208,9 +215,15 @@ __device__ __forceinline__ bool tile_out(const Params &p, const CUtensorMap *tma
             float v[16], sb[16], bias[16], r[16];
             if (R && row < g.M)
                 load_row(r, R + (long)row * g.ldc + at, g.N - at, whole && p.al_r);
-            load_cols(sb, g.sb, at, g.N, whole);
-            if (g.bias)
-                load_cols(bias, g.bias, at, g.N, whole);
+            if (SHARED) {
+                load_cols(sb, cols, at - n0, BN, true);
+                load_cols(bias, cols + BN, at - n0, BN, true);
+            }
+            else {
+                load_cols(sb, g.sb, at, g.N, whole);
+                if (g.bias)
+                    load_cols(bias, g.bias, at, g.N, whole);
+            }
             tmem_ld16(acc + c0 + 16 * h, v);
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
@@ -220,7 +233,7 @@ __device__ __forceinline__ bool tile_out(const Params &p, const CUtensorMap *tma
                                       pair(sa), pair(0.0f));
                 const float2 x = act2<ACT>(
                     fma2(y, make_float2(sb[j], sb[j + 1]),
-                         g.bias ? make_float2(bias[j], bias[j + 1]) : pair(0.0f)),
+                         SHARED || g.bias ? make_float2(bias[j], bias[j + 1]) : pair(0.0f)),
                     g.slope);
                 v[j] = x.x;
                 v[j + 1] = x.y;
@@ -241,12 +254,13 @@ __device__ __forceinline__ bool tile_out(const Params &p, const CUtensorMap *tma
             continue;
         }
         __syncwarp();
-        // Rows without a tensor map: 32 / COLS rows at a time, lane = column.
+        // Rows without a tensor map: lane = column, several rows at a time where
+        // they are short.
+        constexpr int E = 16 / (int)sizeof(TC);
         const int c = lane % COLS;
         if (col + c < g.N)
             for (int r = lane / COLS; r < 32 && m0 + r < g.M; r += 32 / COLS)
-                C[(long)(m0 + r) * g.ldc + col + c] =
-                    ((const TC *)chunk(cst, r, c * (int)sizeof(TC) / 16))[c % (16 / (int)sizeof(TC))];
+                C[(long)(m0 + r) * g.ldc + col + c] = ((const TC *)chunk(cst, r, c / E))[c % E];
     }
     // Each tcgen05.ld has waited: the accumulator may be written again.
     fence_before();
@@ -341,9 +355,10 @@ tc_i8_k(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUten
         int lt = 0;
         for (int t = blockIdx.x; t < ntiles; t += gridDim.x, lt++) {
             const int buf = lt % 2;
-            if (!tile_out<BN, ACT, TC>(p, &tma_c, cst, tmem + (uint32_t)(buf * acc_cols<BN>()),
+            if (!tile_out<BN, false, ACT, TC>(p, &tma_c, cst, tmem + (uint32_t)(buf * acc_cols<BN>()),
                                        &s.acc_full[buf], lt / 2 & 1, (t % tiles_m) * BM,
-                                       (t / tiles_m) * BN, warp % 4, (warp - 2) / 4, lane))
+                                       (t / tiles_m) * BN, warp % 4, (warp - 2) / 4, lane,
+                                       nullptr))
                 break;
             if (lane == 0)
                 mbar_arrive(&s.acc_empty[buf]);
@@ -360,49 +375,303 @@ tc_i8_k(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUten
     }
 }
 
-template <int BN, int ACT, typename TC>
-bool run(cudaStream_t st, int grid, const CUtensorMap &ma, const CUtensorMap &mb,
-         const CUtensorMap &mc, const Params &p)
+// ------------------------------------------------------------- CTA pairs
+//
+// 256 x 256 tiles by two CTAs of a cluster (tcgen05 cta_group::2): each holds 128
+// rows of A, half the rows of B and the sums of its 128 rows; the tensor cores
+// of both read B from both. Per product that is a third less shared memory
+// and L2 traffic than the 128 x 256 tile's, which saves power (these kernels
+// run at the power limit: 25616 x 4096 x 1024 at about 1.3 GHz of 1.9), and
+// leaves room for five stages and the columns' scales.
+// The roles are those above, in each CTA; the first of the pair (the leader)
+// alone issues the products, for both:
+//   full[s]      the leader's: both CTAs' loads of a stage complete on it;
+//   empty[s]     each CTA's own, arrived at in both by the leader's commit;
+//   acc_full     likewise;
+//   acc_empty    the leader's: the epilogue warps of both CTAs arrive.
+constexpr int PAIR_ST = 5, PAIR_BN = 256;
+
+struct PairSmem {
+    alignas(1024) unsigned char a[PAIR_ST][BM * BK];
+    alignas(1024) unsigned char b[PAIR_ST][PAIR_BN / 2 * BK];
+    alignas(1024) unsigned char cst[EPI_WARPS][32 * ROW];
+    alignas(16) float cols[2][2 * PAIR_BN];
+    uint64_t full[PAIR_ST], empty[PAIR_ST], acc_full[2], acc_empty[2];
+    uint32_t tmem;
+};
+
+__device__ __forceinline__ uint32_t cta_rank()
 {
-    const size_t smem = sizeof(Smem<BN>) + 1024;
-    static unsigned done = 0;
-    if (!smem_opt_in((const void *)tc_i8_k<BN, ACT, TC>, smem, &done))
-        return false;
-    launch_chained(tc_i8_k<BN, ACT, TC>, grid, NTHREADS, smem, st, ma, mb, mc, p);
-    return true;
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
 }
 
-template <int BN, typename TC>
+// The cluster address of a barrier of the pair's leader.
+__device__ __forceinline__ uint32_t of_leader(const uint64_t *bar)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(su32(bar)));
+    return r;
+}
+
+// A box into this CTA's shared memory that completes on a barrier of the pair.
+__device__ __forceinline__ void pair_load_2d(void *dst, const CUtensorMap *map, uint32_t bar, int x,
+                                             int y)
+{
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::"
+                 "bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(su32(dst)),
+                 "l"((uint64_t)map), "r"(bar), "r"(x), "r"(y)
+                 : "memory");
+}
+
+__device__ __forceinline__ void pair_mma_i8(uint32_t tmem, uint64_t da, uint64_t db,
+                                            uint32_t idesc, uint32_t accum)
+{
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
+                 "l"(da), "l"(db), "r"(idesc), "r"(accum));
+}
+
+// The issued products done: arrives at the barrier's place in both CTAs.
+__device__ __forceinline__ void pair_commit(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::"
+                 "cluster.b64 [%0], %1;" ::"r"(su32(bar)),
+                 "h"((uint16_t)3)
+                 : "memory");
+}
+
+__device__ __forceinline__ void pair_arrive(uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+                 : "memory");
+}
+
+// mbar_wait for arrivals from the other CTA.
+__device__ __forceinline__ bool pair_wait(uint64_t *b, uint32_t parity, int code)
+{
+    uint64_t t0 = 0;
+    for (;;) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\t"
+                     "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+                     "selp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok)
+                     : "r"(su32(b)), "r"(parity)
+                     : "memory");
+        if (ok)
+            return true;
+        if (!t0)
+            t0 = gtime();
+        else if (gtime() - t0 > 2000000000ull) {
+            atomicCAS(&g_error, 0, code);
+            return false;
+        }
+    }
+}
+
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                     : "memory");
+}
+
+template <int ACT, typename TC>
+__global__ void __launch_bounds__(NTHREADS, 1) __cluster_dims__(2, 1, 1)
+tc_i8_pair_k(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
+             const __grid_constant__ CUtensorMap tma_c, const Params p)
+{
+    constexpr int ST = PAIR_ST, BN = PAIR_BN;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    PairSmem &s =
+        *reinterpret_cast<PairSmem *>(smem_raw + ((1024u - (su32(smem_raw) & 1023u)) & 1023u));
+    const I8Gemm &g = p.g;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int rank = (int)cta_rank(), pairs = (int)gridDim.x / 2;
+    const int nk = (g.K + BK - 1) / BK;
+    const int tiles_m = (g.M + 2 * BM - 1) / (2 * BM);
+    const int ntiles = tiles_m * ((g.N + BN - 1) / BN);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < ST; i++) {
+            mbar_init(&s.full[i], 1);
+            mbar_init(&s.empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&s.acc_full[i], 1);
+            mbar_init(&s.acc_empty[i], 2 * EPI_WARPS);
+        }
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         su32(&s.tmem)),
+                     "r"(512u));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    after_previous();
+    fence_before();
+    __syncthreads();
+    cluster_sync();
+    fence_after();
+    const uint32_t tmem = s.tmem;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int t = blockIdx.x / 2; t < ntiles && ok; t += pairs) {
+                const int m0 = (t % tiles_m) * 2 * BM + rank * BM;
+                const int n0 = (t / tiles_m) * BN + rank * (BN / 2);
+                for (int kb = 0; kb < nk; kb++, it++) {
+                    const int st = it % ST;
+                    if (it >= ST && !pair_wait(&s.empty[st], ((it / ST) - 1) & 1, 71)) {
+                        ok = false;
+                        break;
+                    }
+                    if (rank == 0)
+                        mbar_expect_tx(&s.full[st], 2 * (BM + BN / 2) * BK);
+                    const uint32_t bar = of_leader(&s.full[st]);
+                    pair_load_2d(s.a[st], &tma_a, bar, kb * BK, m0);
+                    pair_load_2d(s.b[st], &tma_b, bar, kb * BK, n0);
+                }
+            }
+        }
+    }
+    else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = idesc_i8(2 * BM, BN);
+            int it = 0, lt = 0;
+            bool ok = true;
+            for (int t = blockIdx.x / 2; t < ntiles && ok; t += pairs, lt++) {
+                const int buf = lt % 2, use = lt / 2;
+                if (use > 0 && !pair_wait(&s.acc_empty[buf], (use - 1) & 1, 74))
+                    break;
+                fence_after();
+                const uint32_t acc = tmem + (uint32_t)(buf * BN);
+                for (int kb = 0; kb < nk; kb++, it++) {
+                    const int st = it % ST;
+                    if (!pair_wait(&s.full[st], (it / ST) & 1, 72)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint64_t da = sw128_desc(su32(s.a[st])), db = sw128_desc(su32(s.b[st]));
+#pragma unroll
+                    for (int k = 0; k < BK / 32; k++)
+                        pair_mma_i8(acc, da + 2 * k, db + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                    pair_commit(&s.empty[st]);
+                }
+                if (ok)
+                    pair_commit(&s.acc_full[buf]);
+            }
+        }
+    }
+    else {
+        unsigned char *cst = s.cst[warp - 2];
+        // Scales and bias of a tile's columns, one value per epilogue thread,
+        // fetched a tile ahead. (Read from global memory by every warp they
+        // were 1.7 of the 6 thousand cycles of an epilogue.) The barrier of
+        // the next tile is behind every read of this one's.
+        const int me = threadIdx.x - 64;
+        auto value = [&](int t) {
+            const int c = (t / tiles_m) * BN + me % BN;
+            const float *from = me < BN ? g.sb : g.bias;
+            return t < ntiles && from && c < g.N ? from[c] : 0.0f;
+        };
+        float next = value(blockIdx.x / 2);
+        bool ok = true;
+        int lt = 0;
+        for (int t = blockIdx.x / 2; t < ntiles; t += pairs, lt++) {
+            const int buf = lt % 2;
+            float *cols = s.cols[buf];
+            cols[me] = next;
+            named_bar(1, 32 * EPI_WARPS);
+            next = value(t + pairs);
+            // (A warp whose wait ran out keeps to the barriers of the others.)
+            ok = ok && tile_out<BN, true, ACT, TC>(
+                           p, &tma_c, cst, tmem + (uint32_t)(buf * BN), &s.acc_full[buf],
+                           lt / 2 & 1, (t % tiles_m) * 2 * BM + rank * BM, (t / tiles_m) * BN,
+                           warp % 4, (warp - 2) / 4, lane, cols);
+            if (ok && lane == 0)
+                pair_arrive(of_leader(&s.acc_empty[buf]));
+        }
+        if (lane == 0)
+            bulk_wait_all();
+    }
+    // Neither CTA leaves while the other's barriers, operands or loads need it.
+    fence_before();
+    __syncthreads();
+    cluster_sync();
+    if (warp == 1) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    }
+}
+
+// The kernel of an activation.
+template <typename F>
+bool with_act(int act, F f)
+{
+    switch (act) {
+    case ACT_GELU:
+        return f(std::integral_constant<int, ACT_GELU>());
+    case ACT_RELU:
+        return f(std::integral_constant<int, ACT_RELU>());
+    case ACT_LEAKY:
+        return f(std::integral_constant<int, ACT_LEAKY>());
+    case ACT_GELU_TANH:
+        return f(std::integral_constant<int, ACT_GELU_TANH>());
+    case ACT_SILU:
+        return f(std::integral_constant<int, ACT_SILU>());
+    }
+    return f(std::integral_constant<int, ACT_NONE>());
+}
+
+// Whether 256-wide tiles go to CTA pairs: for deep products (8192 x 8192 x
+// 8192 417 us in pairs, 440 without; 25616 x 1024 x 4096 140 and 148; 3202 x
+// 1024 x 4096 22.8 and 24.1). In shallow ones the epilogue leads, and a pair
+// waits for the slower of its two (25616 x 4096 x 1024 145 and 141).
+bool pair_pays(const I8Gemm &g) { return g.M > BM && g.K >= 2048; }
+
+// PAIR: the kernel of CTA pairs (BN 256).
+template <int BN, bool PAIR, typename TC>
 bool launch(cudaStream_t st, const I8Gemm &g, int sms)
 {
     CUtensorMap ma, mb, mc = {};
     Params p;
     p.g = g;
     if (!make_map_rows(&ma, g.A, 1, g.M, g.K, g.lda, BK, BM, 128) ||
-        !make_map_rows(&mb, g.B, 1, g.N, g.K, g.ldb, BK, BN, 128))
+        !make_map_rows(&mb, g.B, 1, g.N, g.K, g.ldb, BK, PAIR ? BN / 2 : BN, 128))
         return false;
     p.tma_out = make_map_rows(&mc, g.C, sizeof(TC), g.M, g.N, g.ldc * (long)sizeof(TC),
                               ROW / (int)sizeof(TC), 32, 64);
     p.al = (((uintptr_t)g.sb | (uintptr_t)g.bias) & 15) == 0;
     p.al_r = ((uintptr_t)g.R & 15) == 0 && g.ldc * (long)sizeof(TC) % 16 == 0;
     p.clean = (long)g.N * (int)sizeof(TC) % 16 == 0;
-    const long tiles = (long)cdiv(g.M, BM) * cdiv(g.N, BN);
+    const long tiles = (long)cdiv(g.M, PAIR ? 2 * BM : BM) * cdiv(g.N, BN);
     if (tiles >= (1L << 31))
         return false;
-    const int grid = (int)(tiles < sms ? tiles : sms);
-    switch (g.act) {
-    case ACT_GELU:
-        return run<BN, ACT_GELU, TC>(st, grid, ma, mb, mc, p);
-    case ACT_RELU:
-        return run<BN, ACT_RELU, TC>(st, grid, ma, mb, mc, p);
-    case ACT_LEAKY:
-        return run<BN, ACT_LEAKY, TC>(st, grid, ma, mb, mc, p);
-    case ACT_GELU_TANH:
-        return run<BN, ACT_GELU_TANH, TC>(st, grid, ma, mb, mc, p);
-    case ACT_SILU:
-        return run<BN, ACT_SILU, TC>(st, grid, ma, mb, mc, p);
-    }
-    return run<BN, ACT_NONE, TC>(st, grid, ma, mb, mc, p);
+    const long most = PAIR ? sms / 2 : sms;
+    const unsigned grid = (unsigned)(tiles < most ? tiles : most) * (PAIR ? 2 : 1);
+    return with_act(g.act, [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
+        static unsigned done = 0;
+        if constexpr (PAIR) {
+            const size_t smem = sizeof(PairSmem) + 1024;
+            if (!smem_opt_in((const void *)tc_i8_pair_k<ACT, TC>, smem, &done))
+                return false;
+            launch_chained(tc_i8_pair_k<ACT, TC>, grid, NTHREADS, smem, st, ma, mb, mc, p);
+        }
+        else {
+            const size_t smem = sizeof(Smem<BN>) + 1024;
+            if (!smem_opt_in((const void *)tc_i8_k<BN, ACT, TC>, smem, &done))
+                return false;
+            launch_chained(tc_i8_k<BN, ACT, TC>, grid, NTHREADS, smem, st, ma, mb, mc, p);
+        }
+        return true;
+    });
 }
 
 template <typename TC>
@@ -412,9 +681,9 @@ bool choose(cudaStream_t st, const I8Gemm &g, int sms)
     // costs its products or, where that is more, its epilogue, and the last
     // epilogue overlaps nothing. 128 bytes of depth take about 600 cycles at
     // any width: an MMA reads its 128 rows of A for 128 cycles, in which it
-    // multiplies up to 256 columns (25616 x 4096 x 1024: 125 us with 256
-    // columns, 144 with 128, 231 with 64; 500 x 500 x 500, where rounds do
-    // not count: 13.5, 10.3 and 8.4).
+    // multiplies up to 256 columns (25616 x 4096 x 1024 in short runs: 125 us
+    // with 256 columns, 144 with 128, 231 with 64; 500 x 500 x 500, where
+    // rounds do not count: 13.5, 10.3 and 8.4).
     const int widths[3] = {256, 128, 64};
     int best = 0;
     double best_t = 0;
@@ -428,9 +697,11 @@ bool choose(cudaStream_t st, const I8Gemm &g, int sms)
             best_t = t;
         }
     }
-    return best == 0   ? launch<256, TC>(st, g, sms)
-           : best == 1 ? launch<128, TC>(st, g, sms)
-                       : launch<64, TC>(st, g, sms);
+    if (best == 0 && pair_pays(g))
+        return launch<256, true, TC>(st, g, sms);
+    return best == 0   ? launch<256, false, TC>(st, g, sms)
+           : best == 1 ? launch<128, false, TC>(st, g, sms)
+                       : launch<64, false, TC>(st, g, sms);
 }
 
 }  // namespace

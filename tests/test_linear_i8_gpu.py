@@ -149,6 +149,16 @@ GEMM = [
     (9, 4096, 200, 16, 1, 1),
     (16, 4100, 144, 0, 0, 0),
     (300, 1, 200, 0, 0, 0),
+    # Wide tiles, and deep ones by CTA pairs: one tile and more of a CTA or pair,
+    # ragged rows, columns and depths.
+    (1000, 4096, 256, 0, 0, 0),
+    (1025, 3850, 130, 16, 0, 2),
+    (2000, 4090, 700, 0, 0, 0),
+    (700, 4096, 2048, 0, 0, 0),
+    (1025, 3850, 2100, 16, 0, 2),
+    (2600, 4352, 2050, 0, 0, 0),
+    (5000, 2100, 2064, 0, 1, 4),
+    (129, 9000, 4000, 0, 0, 0),
 ]
 
 
@@ -173,10 +183,11 @@ def test_gemm(dev, shape, t):
 @pytest.mark.gpu
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("kind", ref.ACTS)
-@pytest.mark.parametrize("M", [5, 300])
-def test_gemm_activations_residual(dev, M, kind, t):
+@pytest.mark.parametrize("shape", [(2, 200, 272), (5, 200, 272), (300, 200, 272), (257, 9000, 2050)],
+                         ids=str)
+def test_gemm_activations_residual(dev, shape, kind, t):
     """Each activation, without a bias, with a residual of its own and in place."""
-    N, K, T = 200, 272, TYPES[t]
+    (M, N, K), T = shape, TYPES[t]
     rng = np.random.default_rng(M + len(kind))
     a, sa, b, sb, _ = operands(rng, M, N, K)
     res = rounded(rng.standard_normal((M, N)), T)
