@@ -100,46 +100,6 @@ __device__ __forceinline__ void load_cols(float v[16], const float *p, int col, 
         v[j] = col + j < n ? p[j] : 0.0f;
 }
 
-// The 16 values of a residual row from R on, zero behind n; whole: they exist
-// and are 16-byte aligned. (Not through the read-only cache: R may be C.)
-__device__ __forceinline__ void load_row(float v[16], const float *R, int n, bool whole)
-{
-    if (whole) {
-#pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-            const float4 x = *(const float4 *)(R + j);
-            v[j] = x.x;
-            v[j + 1] = x.y;
-            v[j + 2] = x.z;
-            v[j + 3] = x.w;
-        }
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 16; j++)
-        v[j] = j < n ? R[j] : 0.0f;
-}
-
-__device__ __forceinline__ void load_row(float v[16], const __nv_bfloat16 *R, int n, bool whole)
-{
-    if (whole) {
-#pragma unroll
-        for (int j = 0; j < 16; j += 8) {
-            const uint4 x = *(const uint4 *)(R + j);
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                v[j + 2 * k] = __uint_as_float(w[k] << 16);
-                v[j + 2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 16; j++)
-        v[j] = j < n ? __bfloat162float(R[j]) : 0.0f;
-}
-
 // Address of 16-byte chunk c of row l of an output block, in its tensor map's
 // 64-byte swizzle.
 __device__ __forceinline__ unsigned char *chunk(unsigned char *blk, int l, int c)
@@ -171,6 +131,34 @@ __device__ __forceinline__ void stage_row(unsigned char *blk, int l, int h, cons
     }
 }
 
+// v += those 16 values of a block.
+__device__ __forceinline__ void add_staged(float v[16], unsigned char *blk, int l, int, const float *)
+{
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const float4 x = *(const float4 *)chunk(blk, l, c);
+        v[4 * c] += x.x;
+        v[4 * c + 1] += x.y;
+        v[4 * c + 2] += x.z;
+        v[4 * c + 3] += x.w;
+    }
+}
+
+__device__ __forceinline__ void add_staged(float v[16], unsigned char *blk, int l, int h,
+                                           const __nv_bfloat16 *)
+{
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        const uint4 x = *(const uint4 *)chunk(blk, l, 2 * h + c);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            v[8 * c + 2 * k] += __uint_as_float(w[k] << 16);
+            v[8 * c + 2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
+        }
+    }
+}
+
 // One epilogue warp's part of a tile: TMEM lanes 32 q .. (rows of the tile from
 // m0 on) and the blocks part, part + 4, ... of columns (from n0 on) of the
 // accumulator acc, which is complete when `full` turns `parity`. SHARED: the
@@ -191,30 +179,49 @@ __device__ __forceinline__ bool tile_out(const Params &p, const CUtensorMap *tma
     const int row = m0 + lane;
     const float sa = row < g.M ? __ldg(g.sa + row) : 0.0f;
     constexpr int STEP = COLS * (EPI_WARPS / 4);
-    // The residual into L2 while the products run: read in place its lines
-    // came from memory one block after the other (15 thousand cycles of
-    // epilogue for a 128 x 256 float tile, 6 without a residual).
+    // The residual's blocks come as the output's leave: 64-byte row segments by
+    // four lanes each, through the staging block, the first while the
+    // products run, each further one a block ahead (and all of them into
+    // L2). Read by one lane per row they took 32 memory lines an
+    // instruction, and 14 thousand cycles of a 128 x 256 float tile.
+    const bool whole = p.al && n0 + BN <= g.N, by_block = R && p.al_r && n0 + BN <= g.N;
+    uint4 next[4];
+    auto fetch = [&](int c0) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = m0 + 8 * i + lane / 4;
+            if (r < g.M)
+                next[i] = *((const uint4 *)(R + (long)r * g.ldc + n0 + c0) + lane % 4);
+        }
+    };
     if (R && row < g.M)
-        for (int c0 = COLS * part; c0 < BN && n0 + c0 < g.N; c0 += STEP)
+        for (int c0 = COLS * part + (by_block ? STEP : 0); c0 < BN && n0 + c0 < g.N; c0 += STEP)
             asm volatile("prefetch.global.L2 [%0];" ::"l"(R + (long)row * g.ldc + n0 + c0));
+    if (by_block && COLS * part < BN)
+        fetch(COLS * part);
     // Decided per warp: the TMEM loads below are warp-collective.
     if (!__all_sync(0xffffffffu, mbar_wait(full, parity, 63)))
         return false;
     fence_after();
     acc += (uint32_t)(32 * q) << 16;
-    const bool whole = p.al && n0 + BN <= g.N;
     for (int c0 = COLS * part; c0 < BN && n0 + c0 < g.N; c0 += STEP) {
         const int col = n0 + c0;
         // The previous store has read the block.
         if (lane == 0)
             bulk_wait_read<0>();
         __syncwarp();
+        if (by_block) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                *(uint4 *)chunk(cst, 8 * i + lane / 4, lane % 4) = next[i];
+            __syncwarp();
+            if (c0 + STEP < BN)
+                fetch(c0 + STEP);
+        }
 #pragma unroll
         for (int h = 0; h < COLS / 16; h++) {
             const int at = col + 16 * h;
-            float v[16], sb[16], bias[16], r[16];
-            if (R && row < g.M)
-                load_row(r, R + (long)row * g.ldc + at, g.N - at, whole && p.al_r);
+            float v[16], sb[16], bias[16];
             if (SHARED) {
                 load_cols(sb, cols, at - n0, BN, true);
                 load_cols(bias, cols + BN, at - n0, BN, true);
@@ -238,10 +245,14 @@ __device__ __forceinline__ bool tile_out(const Params &p, const CUtensorMap *tma
                 v[j] = x.x;
                 v[j + 1] = x.y;
             }
-            if (R && row < g.M)
+            if (by_block)
+                add_staged(v, cst, lane, h, (const TC *)nullptr);
+            else if (R && row < g.M) {
 #pragma unroll
                 for (int j = 0; j < 16; j++)
-                    v[j] += r[j];
+                    if (at + j < g.N)
+                        v[j] += ldf(R + (long)row * g.ldc + at + j);
+            }
             stage_row(cst, lane, h, v, (TC *)nullptr);
         }
         if (p.tma_out && (col + COLS <= g.N || p.clean)) {
