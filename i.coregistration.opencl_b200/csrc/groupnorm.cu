@@ -63,15 +63,17 @@ struct GroupNorm {
     int cols, pitch;      // a group's entries per row lane, entries between lanes
     Div by_slots, by_per, by_C;
     int keep, ring;       // vectors a thread keeps, places of the ring (RING or 0)
-    int merged;           // entries per thread and group, not per channel
-    float2 *work;         // grid teams: 2 x groups x team (mean, M2)
+    int merged;           // neighbouring channels of a thread in one entry
+    int simple;           // all of a thread's, and gamma and beta 16-byte aligned
+    int batch;            // grid teams: images at a time, a team each
+    float2 *work;         // grid teams: 2 x batch x groups x team (mean, M2)
 };
 
 constexpr int MAX_THREADS = 512;
 // Vectors of a thread in flight: 8 x 512 x 16 bytes per multiprocessor cover
 // the memory's latency at its full rate (about 45 KB) with some to spare.
 constexpr int RING = 8;
-constexpr int MAX_TEAM = 256; // blocks of a grid team the work buffer holds
+constexpr int MAX_TEAM = 160; // blocks of a grid team the work buffer holds
 
 
 // V values as they lie in memory: 16 bytes, or one value.
@@ -370,6 +372,30 @@ __device__ __forceinline__ void apply(const GroupNorm &p, const TX *x, TY *y, co
     }
 }
 
+// Entries (mean, M2) of K neighbouring of a thread's V channels each, which
+// have n values each.
+template <int V, int K>
+__device__ __forceinline__ void merge(float2 *to, const float mean[V], const float m2[V], float n)
+{
+#pragma unroll
+    for (int e = 0; e < V; e += K) {
+        float m = mean[e], q = m2[e];
+        if (K > 1) {
+#pragma unroll
+            for (int k = 1; k < K; k++)
+                m += mean[e + k];
+            m *= 1.0f / K;
+            q = 0.0f;
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                const float d = mean[e + k] - m;
+                q += fmaf(n * d, d, m2[e + k]);
+            }
+        }
+        to[e / K] = make_float2(m, q);
+    }
+}
+
 // How a warp walks a group's entries: lane l takes the columns l % pw, + pw, ...
 // of `cols`, and of each the rows l / pw, + 32 / pw, ... (pw a power of two), so
 // that the loops hold no division. visit(column, row).
@@ -395,7 +421,8 @@ groupnorm_k(const __grid_constant__ GroupNorm p)
     float2 *mine = entry + p.pitch * p.lanes; // the block's (mean, M2) per group
     float2 *team = mine + p.gs;                   // the team's (mean, 1 / sigma)
     // (The blocks of a cluster team are a power of two.)
-    const int rank = GRID ? (int)blockIdx.x : (int)(blockIdx.x & (p.team - 1));
+    const int which = GRID ? (int)blockIdx.x / p.team : 0; // the team's image of a batch
+    const int rank = GRID ? (int)blockIdx.x - which * p.team : (int)(blockIdx.x & (p.team - 1));
     const int slice = GRID ? 0 : (int)blockIdx.x >> (31 - __clz(p.team));
     const int g0 = slice * p.gs, gn = min(p.gs, p.groups - g0); // its groups
     const int c0 = g0 * p.per;
@@ -424,7 +451,13 @@ groupnorm_k(const __grid_constant__ GroupNorm p)
 
     if (!GRID)
         after_previous();
-    for (int img = GRID ? 0 : (int)blockIdx.y; img < p.nimg; img += GRID ? 1 : p.nimg) {
+    for (int img0 = GRID ? 0 : (int)blockIdx.y; img0 < p.nimg; img0 += GRID ? p.batch : p.nimg) {
+        const int img = img0 + which;
+        // (A last batch may have fewer images than teams.)
+        if (GRID && img >= p.nimg) {
+            cg::this_grid().sync();
+            continue;
+        }
         const TX *x = (const TX *)p.X + img * p.sx + c0;
         TY *y = (TY *)p.Y + img * p.sy + c0;
 
@@ -432,21 +465,40 @@ groupnorm_k(const __grid_constant__ GroupNorm p)
         sums_begin<TX, V>(p, x, at, kept);
         float ga[V], be[V];
         int gi[V]; // the elements' groups
+        if (V > 1 && p.simple) {
+            // Whole vectors of one group, gamma and beta aligned as the map is.
+            const int g = active ? p.by_per(at.j0) : 0;
 #pragma unroll
-        for (int e = 0; e < V; e++) {
-            const int j = at.j0 + e, c = p.R > 1 ? j - p.by_C(j) * p.C : j;
-            const bool in = active && j < width;
-            gi[e] = in ? p.by_per(c) : 0;
-            ga[e] = in && p.g ? __ldg(p.g + c0 + c) : 1.0f;
-            be[e] = in && p.g ? __ldg(p.b + c0 + c) : 0.0f;
+            for (int e = 0; e < V; e++) {
+                gi[e] = g;
+                ga[e] = 1.0f;
+                be[e] = 0.0f;
+            }
+            if (p.g && active)
+#pragma unroll
+                for (int e = 0; e < V; e += 4) {
+                    const float4 u = __ldg((const float4 *)(p.g + c0 + at.j0 + e)),
+                                 v = __ldg((const float4 *)(p.b + c0 + at.j0 + e));
+                    ga[e] = u.x, ga[e + 1] = u.y, ga[e + 2] = u.z, ga[e + 3] = u.w;
+                    be[e] = v.x, be[e + 1] = v.y, be[e + 2] = v.z, be[e + 3] = v.w;
+                }
         }
+        else
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const int j = at.j0 + e, c = p.R > 1 ? j - p.by_C(j) * p.C : j;
+                const bool in = active && j < width;
+                gi[e] = in ? p.by_per(c) : 0;
+                ga[e] = in && p.g ? __ldg(p.g + c0 + c) : 1.0f;
+                be[e] = in && p.g ? __ldg(p.b + c0 + c) : 0.0f;
+            }
         {
             float x0[V], s1[V], s2[V];
             sums<TX, V>(p, x, at, x0, s1, s2, kept);
-            // 2. Entries (mean, M2): one per thread where its vector lies in
-            // one group, else one per channel.
+            // 2. Entries (mean, M2): of p.merged neighbouring channels that lie in
+            // one group (all of a thread's, four, two or one).
             if (active) {
-const float i0 = at.cnt > 0 ? 1.0f / (float)at.cnt : 0.0f,
+                const float i0 = at.cnt > 0 ? 1.0f / (float)at.cnt : 0.0f,
                             i1 = at.tail > 0 ? 1.0f / (float)(at.cnt + 1) : 0.0f;
 #pragma unroll
                 for (int e = 0; e < V; e++) {
@@ -454,59 +506,53 @@ const float i0 = at.cnt > 0 ? 1.0f / (float)at.cnt : 0.0f,
                     s2[e] = fmaxf(s2[e] - s1[e] * m, 0.0f);
                     s1[e] = x0[e] + m;
                 }
-                if (p.merged) {
-                    float m = 0.0f, q = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < V; e++)
-                        m += s1[e];
-                    m *= 1.0f / V;
-#pragma unroll
-                    for (int e = 0; e < V; e++) {
-                        const float d = s1[e] - m;
-                        q += fmaf((float)at.cnt * d, d, s2[e]);
-                    }
-                    entry[row * p.pitch + slot] = make_float2(m, q);
-                }
-                else {
-#pragma unroll
-                    for (int e = 0; e < V; e++)
-                        entry[row * p.pitch + at.j0 + e] = make_float2(s1[e], s2[e]);
-                }
+                float2 *to = entry + row * p.pitch;
+                const float n = (float)at.cnt;
+                if (V > 1 && p.merged == V)
+                    merge<V, V>(to + slot, s1, s2, n);
+                else if (V == 8 && p.merged == 4)
+                    merge<V, 4>(to + slot * 2, s1, s2, n);
+                else if (V > 2 && p.merged == 2)
+                    merge<V, 2>(to + slot * (V / 2), s1, s2, n);
+                else
+                    merge<V, 1>(to + at.j0, s1, s2, n);
             }
         }
         __syncthreads();
-        float2 *out = GRID ? p.work + (size_t)(img & 1) * p.groups * p.team : nullptr;
+        float2 *out = GRID ? p.work + (size_t)((img0 / p.batch & 1) * p.batch + which) *
+                                          p.groups * p.team
+                           : nullptr;
         const float here = (float)(((long)min((long)sr1 * p.R, (long)p.HW) - (long)sr0 * p.R) * p.per);
         // Entries of a group: p.cols in a row lane, p.pitch between row lanes;
         // each of (base, or base + 1 in the first `more` row lanes) pixels of
-        // `each` channels, one less where the map's last super row ends.
-        const float each = p.merged ? (float)V : 1.0f;
+        // p.merged channels, one less where the map's last super row ends.
+        // Sums about the group's first entry, one of those added.
         for (int g = warp; g < gn; g += nwarp) {
-            auto visit = [&](auto f) {
-                walk(p.cols, p.lanes, lane, [&](int c, int r) {
-                    int j = g * p.cols + c, n = base + (r < more);
-                    if (!p.merged) {
-                        const int q = p.by_per(c);
-                        j = q * p.C + g * p.per + (c - q * p.per);
-                        n -= r == last && j >= p.wlast;
-                    }
-                    f(entry[r * p.pitch + j], (float)n * each);
-                });
-            };
-            float s = 0.0f;
-            visit([&](float2 v, float w) { s = fmaf(v.x, w, s); });
-            const float m = here > 0.0f ? warp_sum(s) / here : 0.0f;
-            s = 0.0f;
-            visit([&](float2 v, float w) {
-                const float d = v.x - m;
-                s += w > 0.0f ? fmaf(w * d, d, v.y) : 0.0f;
+            const float m0 = entry[p.R > 1 ? g * p.per : g * p.cols].x;
+            float a = 0.0f, q = 0.0f;
+            walk(p.cols, p.lanes, lane, [&](int c, int r) {
+                int j = g * p.cols + c, n = base + (r < more);
+                if (p.R > 1) {
+                    const int k = p.by_per(c);
+                    j = k * p.C + g * p.per + (c - k * p.per);
+                    n -= r == last && j >= p.wlast;
+                }
+                const float2 v = entry[r * p.pitch + j];
+                const float w = (float)(n * p.merged), d = v.x - m0;
+                if (n > 0) {
+                    a = fmaf(w, d, a);
+                    q += fmaf(w * d, d, v.y);
+                }
             });
-            s = warp_sum(s);
+            a = warp_sum(a);
+            q = warp_sum(q);
             if (lane == 0) {
+                const float m = here > 0.0f ? a / here : 0.0f;
+                const float2 s = make_float2(m0 + m, fmaxf(q - a * m, 0.0f));
                 if (GRID)
-                    out[(size_t)g * p.team + rank] = make_float2(m, s);
+                    out[(size_t)g * p.team + rank] = s;
                 else
-                    mine[g] = make_float2(m, s);
+                    mine[g] = s;
             }
         }
         if (GRID)
@@ -526,20 +572,25 @@ const float i0 = at.cnt > 0 ? 1.0f / (float)at.cnt : 0.0f,
             const long a = (long)run_start(p, t) * p.R, b = (long)run_start(p, t + 1) * p.R;
             n[k] = t < p.team ? (float)((min(b, (long)p.HW) - a) * p.per) : 0.0f;
         }
-        for (int g = warp; g < gn; g += nwarp) {
-            float2 part[NP];
-            float s = 0.0f;
+        auto parts = [&](int g, float2 part[NP]) {
 #pragma unroll
             for (int k = 0; k < NP; k++) {
                 const int t = lane + 32 * k;
                 part[k] = make_float2(0.0f, 0.0f);
-                if (t < p.team) {
+                if (t < p.team && g < gn) {
                     if (GRID)
                         part[k] = __ldcg(&out[(size_t)g * p.team + t]);
                     else
                         part[k] = p.team > 1 ? cg::this_cluster().map_shared_rank(mine, t)[g] : mine[g];
                 }
             }
+        };
+        float2 part[NP];
+        parts(warp, part);
+        for (int g = warp; g < gn; g += nwarp) {
+            float2 next[NP];
+            parts(g + nwarp, next);
+            float s = 0.0f;
 #pragma unroll
             for (int k = 0; k < NP; k++)
                 s = fmaf(part[k].x, n[k], s);
@@ -550,6 +601,7 @@ const float i0 = at.cnt > 0 ? 1.0f / (float)at.cnt : 0.0f,
                 const float d = part[k].x - m;
                 if (n[k] > 0.0f)
                     s += fmaf(n[k] * d, d, part[k].y);
+                part[k] = next[k];
             }
             s = warp_sum(s) / N;
             if (lane == 0)
@@ -671,10 +723,16 @@ bool launch(cudaStream_t st, GroupNorm p, int sms)
         p.R *= 2;
     p.nsr = (p.HW + p.R - 1) / p.R;
     p.wlast = (p.HW - (p.nsr - 1) * p.R) * p.C;
-    p.merged = p.R == 1 && p.per % V == 0;
+    p.batch = 1;
+    p.merged = p.R > 1                       ? 1
+               : p.per % V == 0              ? V
+               : p.per % 4 == 0 && V == 8    ? 4
+               : p.per % 2 == 0 && V > 2     ? 2
+                                             : 1;
+    p.simple = p.merged == V && (((uintptr_t)p.g | (uintptr_t)p.b) & 15) == 0;
     p.by_per.set(p.per < 65536 ? p.per : 65535);
     p.by_C.set(p.C < 65536 ? p.C : 65535); // (wider maps have R = 1)
-    p.cols = p.merged ? p.per / V : p.per * p.R;
+    p.cols = p.R > 1 ? p.per * p.R : p.per / p.merged;
     // Slices of whole groups whose vectors start aligned: the smallest unit.
     int unit = 1;
     while (unit < p.groups && (p.R > 1 || (long)unit * p.per % V))
@@ -685,9 +743,23 @@ bool launch(cudaStream_t st, GroupNorm p, int sms)
     if (unit > gmax && p.groups > gmax)
         return false;
 
-    // Cluster teams: every slice width and team size; time in units of bytes
-    // moved at the rate of one of `sms` busy multiprocessors.
+    // Every slice width and team size, and grid teams; times in microseconds by
+    // a model: memory at 6.5 MB per microsecond over the whole device, at most
+    // 1.5 times an even share per multiprocessor; what is read again from L2
+    // at twice that where the maps under way are below 110 MB, else from memory,
+    // which costs 1.8 times its bytes over the grid and 2.6 in clusters, whose
+    // passes mix; 0.7 of the rate for slices, which leave parts of memory's
+    // rows; and the chain of barrier and statistics (4 us in a cluster, 9
+    // over the grid). Measured: two maps of 864 x 864 x 64 bfloat16
+    // one after the other 89 us, at a time 97; five of 71428 x 252 float32 170
+    // and 186 (two at a time), in clusters 223; six of 46656 x 64 bfloat16
+    // 56 and 29 (three at a time), in clusters 26.
     const double esz = sizeof(TX), eout = sizeof(TY);
+    auto model = [&](double elems, double again, double blocks, double far) {
+        const double f = blocks * 1.5 < sms ? blocks * 1.5 / sms : 1.0;
+        const double reread = elems * again * esz * (elems * esz < 110e6 ? 0.5 : far);
+        return (elems * (esz + eout) + reread) / (6.5e6 * f);
+    };
     GroupNorm best = p;
     double best_t = 1e30;
     bool best_grid = false;
@@ -712,7 +784,7 @@ bool launch(cudaStream_t st, GroupNorm p, int sms)
         q.by_slots.set(q.slots);
         // The rows that a warp reads at once (walk) start cols entries apart in
         // the 16 of a pass over the banks, not all in the same.
-        q.pitch = q.merged ? q.slots : q.slots * V;
+        q.pitch = q.slots * V / q.merged;
         if (q.cols < 16)
             while (q.pitch % 16 != (q.cols <= 1 ? 1 : q.cols <= 2 ? 2 : q.cols <= 4 ? 4 : 8))
                 q.pitch++;
@@ -745,12 +817,11 @@ bool launch(cudaStream_t st, GroupNorm p, int sms)
             const double ctas = (double)p.nimg * q.slices * team;
             const double room = team * (double)clusters_of(fn, team, sms);
             const double waves = ctas > room ? (double)(long)((ctas + room - 1) / room) : 1.0;
-            const double n = (double)p.nsr / team * width / esz;
-            const double again = need > q.keep ? n * (1.0 - (double)(q.keep + q.ring) / need) * esz : 0.0;
-            // One multiprocessor moves about 1.5 times its share of the whole
-            // device's rate when few are busy.
-            const double busy = ctas < room ? (ctas > room / 1.5 ? ctas / room : 1.0 / 1.5) : 1.0;
-            const double t = waves * (n * (esz + eout) + again) * busy + 40000.0;
+            const double busy = ctas < room ? ctas : room;
+            const double n = (double)p.nsr / team * width / esz; // elements of a block
+            const double again = need > q.keep ? 1.0 - (double)(q.keep + q.ring) / need : 0.0;
+            const double t =
+                waves * (model(busy * n, again, busy, 2.6) / (q.slices > 1 ? 0.7 : 1.0) + 4.0);
             if (t < best_t) {
                 best_t = t;
                 best = q;
@@ -758,20 +829,24 @@ bool launch(cudaStream_t st, GroupNorm p, int sms)
             }
         }
     }
-    if (p.groups <= gmax && p.nsr >= 4 * sms) {
+    const int all = sms < MAX_TEAM ? sms : MAX_TEAM;
+    for (int batch = 1; p.groups <= gmax && batch <= p.nimg && batch <= 8; batch++) {
         GroupNorm q = p;
-        const int team = sms < MAX_TEAM ? sms : MAX_TEAM;
+        const int team = all / batch;
+        if (p.nsr < 4 * team)
+            continue;
         const long need = geometry(q, p.groups, team);
-        if (need >= 0) {
-            const double n = (double)p.HW / team * p.C;
-            const double again =
-                need > q.keep ? n * (1.0 - (double)(q.keep + q.ring) / need) * esz : 0.0;
-            const double t = p.nimg * (n * (esz + eout) + again + 120000.0);
-            if (t < best_t) {
-                best_t = t;
-                best = q;
-                best_grid = true;
-            }
+        if (need < 0)
+            continue;
+        q.batch = batch;
+        const double n = (double)p.HW * p.C * batch;
+        const double again = need > q.keep ? 1.0 - (double)(q.keep + q.ring) / need : 0.0;
+        const double t = (double)((p.nimg + batch - 1) / batch) *
+                         (model(n, again, all, 1.8) + 9.0);
+        if (t < best_t) {
+            best_t = t;
+            best = q;
+            best_grid = true;
         }
     }
     if (best_t >= 1e30)
@@ -792,7 +867,7 @@ bool launch(cudaStream_t st, GroupNorm p, int sms)
     cfg.attrs = at;
     cfg.numAttrs = 1;
     if (best_grid) {
-        cfg.gridDim = dim3(best.team);
+        cfg.gridDim = dim3(best.team * best.batch);
         at[0].id = cudaLaunchAttributeCooperative;
         at[0].val.cooperative = 1;
     }
@@ -852,7 +927,7 @@ bool map_view(View *v, const char *fn, const char *what, const struct opnd &m, i
 
 extern "C" size_t ops_groupnorm_cl_bytes(int nimg, long HW, int C, int groups)
 {
-    // Two images' (mean, M2) per group and block of a team of the whole grid.
+    // Two batches' (mean, M2) per group and block of the whole grid.
     return nimg <= 0 || HW <= 0 || C <= 0 || groups <= 0
                ? 0
                : (size_t)2 * groups * MAX_TEAM * sizeof(float2);

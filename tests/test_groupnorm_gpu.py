@@ -92,6 +92,15 @@ SHAPES = [
     (40, 5, 8, 2, (0, 8, 0), (0, 8, 0)),
     (2, 130000, 8, 4, (0, 8, 0), (0, 8, 0)),
     (1, 90001, 64, 16, (0, 64, 0), (0, 64, 0)),
+    # Several images at a time over the whole grid, the last batch not full;
+    # channels merged by four, two and none; rows in twos, fours and eights.
+    (3, 60001, 32, 8, (0, 32, 0), (0, 32, 0)),
+    (5, 30007, 64, 32, (0, 64, 2), (0, 64, 0)),
+    (3, 50001, 36, 9, (0, 36, 0), (0, 36, 0)),
+    (2, 70003, 34, 17, (0, 34, 0), (0, 34, 0)),
+    (4, 9001, 204, 34, (0, 204, 0), (0, 204, 0)),
+    (1, 40009, 63, 7, (0, 63, 0), (0, 63, 0)),
+    (3, 5, 21, 7, (0, 21, 0), (0, 21, 0)),
 ]
 
 
