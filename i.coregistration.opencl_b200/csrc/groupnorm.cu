@@ -408,8 +408,9 @@ __device__ __forceinline__ void walk(int cols, int lanes, int lane, F visit)
             visit(c, r);
 }
 
-// GRID: one team of all blocks (a cooperative launch), images one after the
-// other; otherwise a team is a cluster, one per image and slice.
+// GRID: all blocks at once (a cooperative launch) in teams of a batch of images,
+// batches one after the other; otherwise a team is a cluster, one per image
+// and slice.
 template <typename TX, typename TY, int V, bool GRID>
 __global__ void __launch_bounds__(MAX_THREADS, 1)
 groupnorm_k(const __grid_constant__ GroupNorm p)
@@ -419,7 +420,7 @@ groupnorm_k(const __grid_constant__ GroupNorm p)
     typename Vec<TX, V>::Kept *kept = (typename Vec<TX, V>::Kept *)smem + tid;
     float2 *entry = (float2 *)(smem + kept_bytes(p, blockDim.x, sizeof(*kept)));
     float2 *mine = entry + p.pitch * p.lanes; // the block's (mean, M2) per group
-    float2 *team = mine + p.gs;                   // the team's (mean, 1 / sigma)
+    float2 *team = mine + p.gs;               // the team's (mean, 1 / sigma)
     // (The blocks of a cluster team are a power of two.)
     const int which = GRID ? (int)blockIdx.x / p.team : 0; // the team's image of a batch
     const int rank = GRID ? (int)blockIdx.x - which * p.team : (int)(blockIdx.x & (p.team - 1));
@@ -477,8 +478,8 @@ groupnorm_k(const __grid_constant__ GroupNorm p)
             if (p.g && active)
 #pragma unroll
                 for (int e = 0; e < V; e += 4) {
-                    const float4 u = __ldg((const float4 *)(p.g + c0 + at.j0 + e)),
-                                 v = __ldg((const float4 *)(p.b + c0 + at.j0 + e));
+                    const float4 u = *(const float4 *)(p.g + c0 + at.j0 + e),
+                                 v = *(const float4 *)(p.b + c0 + at.j0 + e);
                     ga[e] = u.x, ga[e + 1] = u.y, ga[e + 2] = u.z, ga[e + 3] = u.w;
                     be[e] = v.x, be[e + 1] = v.y, be[e + 2] = v.z, be[e + 3] = v.w;
                 }
@@ -489,8 +490,8 @@ groupnorm_k(const __grid_constant__ GroupNorm p)
                 const int j = at.j0 + e, c = p.R > 1 ? j - p.by_C(j) * p.C : j;
                 const bool in = active && j < width;
                 gi[e] = in ? p.by_per(c) : 0;
-                ga[e] = in && p.g ? __ldg(p.g + c0 + c) : 1.0f;
-                be[e] = in && p.g ? __ldg(p.b + c0 + c) : 0.0f;
+                ga[e] = in && p.g ? p.g[c0 + c] : 1.0f;
+                be[e] = in && p.g ? p.b[c0 + c] : 0.0f;
             }
         {
             float x0[V], s1[V], s2[V];

@@ -33,7 +33,7 @@ struct RowScale {
         inv = half = 0.0f;
         if (amax < 0x7f800000u) {
             s = __fdiv_rn(__uint_as_float(amax), 127.0f);
-            // Below 2^-90 1 / s could overflow and s be denormal: slow().
+            // Below 2^-90 1 / s could overflow and s be denormal: quotient().
             if (s >= 0x1p-90f) {
                 inv = __fdiv_rn(1.0f, s);
                 half = 0.5f * s;
@@ -287,7 +287,7 @@ i8_empty_k(const I8Gemm g)
     const long n = (long)g.M * g.N;
     for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long)gridDim.x * 256) {
         const long m = e / g.N, c = e - m * g.N, at = m * g.ldc + c;
-        float v = act_any(scaled(0, g.sa ? g.sa[m] : 0.0f, g.sb[c], g.bias ? g.bias[c] : 0.0f),
+        float v = act_any(scaled(0, g.sa[m], g.sb[c], g.bias ? g.bias[c] : 0.0f),
                           g.act, g.slope);
         if (g.R)
             v += ldf((const TC *)g.R + at);
@@ -437,14 +437,14 @@ i8_few_k(const I8Gemm g, const Tokens x, int split)
     // The epilogue's thread: channel c, tokens m0, m0 + THREADS / channels, ...
     const int c = threadIdx.x % channels, m0 = threadIdx.x / channels;
     const bool out = c0 + c < g.N;
-    const float sb = out ? __ldg(g.sb + c0 + c) : 0.0f;
-    const float bias = out && g.bias ? __ldg(g.bias + c0 + c) : 0.0f;
+    const float sb = out ? g.sb[c0 + c] : 0.0f;
+    const float bias = out && g.bias ? g.bias[c0 + c] : 0.0f;
     if constexpr (FLOATS) {
         __syncthreads();
         quant_tokens<TX>(x, g.M, g.K, tok, scale, amax);
     }
     else if (threadIdx.x < g.M) {
-        scale[threadIdx.x] = __ldg(g.sa + threadIdx.x);
+        scale[threadIdx.x] = g.sa[threadIdx.x];
     }
     int sum[NT][4] = {};
     for (; k - kk < g.K; k += U * step) {
@@ -545,14 +545,14 @@ i8_dot_k(const I8Gemm g, const Tokens x, int split)
             a[u][r] = load16(w[r], k + u * step, g.K);
     const int c = threadIdx.x % channels, m0 = threadIdx.x / channels;
     const bool out = m0 < g.M && c0 + c < g.N;
-    const float sb = out ? __ldg(g.sb + c0 + c) : 0.0f;
-    const float bias = out && g.bias ? __ldg(g.bias + c0 + c) : 0.0f;
+    const float sb = out ? g.sb[c0 + c] : 0.0f;
+    const float bias = out && g.bias ? g.bias[c0 + c] : 0.0f;
     if constexpr (FLOATS) {
         __syncthreads();
         quant_tokens<TX>(x, g.M, g.K, tok, scale, amax);
     }
     else if (threadIdx.x < g.M) {
-        scale[threadIdx.x] = __ldg(g.sa + threadIdx.x);
+        scale[threadIdx.x] = g.sa[threadIdx.x];
     }
     int acc[DOT_ROWS][MT] = {};
     for (; k - 16 * lane < g.K; k += U * step) {
@@ -687,10 +687,6 @@ void gemm_i8(const struct ocl_backend *ocl, const I8Gemm &g)
         fail("8-bit product of %d x %d x %d: the tensor cores refused the operands", g.M, g.N, g.K);
 }
 
-}  // namespace
-
-namespace {
-
 // -------------------------------------------------------------- arguments
 
 // Rows and columns whose tile indexes stay within 31 bits.
@@ -714,9 +710,8 @@ bool i8_view(View *v, const char *fn, const char *what, const struct opnd &m, lo
 // scales, bias, output and residual.
 bool product_args(const char *fn, I8Gemm *g, int M, int N, int K, const struct opnd &B, cl_mem sb,
                   cl_mem bias, const struct opnd &C, int ctype, cl_mem R, long roff, int act,
-                  float slope, View *out, View in[4], int *nin)
+                  float slope, View *out, View *res, View *in, int *nin)
 {
-    View r;
     if (M < 0 || N < 0 || K < 0 || K > OPS_I8_MAX_K || M > I8_MAX_ROWS || N > I8_MAX_ROWS) {
         fail("%s: %d x %d x %d (depth 0..%d)", fn, M, N, K, OPS_I8_MAX_K);
         return false;
@@ -742,13 +737,13 @@ bool product_args(const char *fn, I8Gemm *g, int M, int N, int K, const struct o
         return false;
     g->R = nullptr;
     if (R) {
-        if (!view_of(&r, fn, "R", R, roff, C.ld, M, N, es))
+        if (!view_of(res, fn, "R", R, roff, C.ld, M, N, es))
             return false;
-        if (!same_view(r, *out) && views_meet(r, *out)) {
+        if (!same_view(*res, *out) && views_meet(*res, *out)) {
             fail("%s: R and C overlap and are not the same", fn);
             return false;
         }
-        g->R = r.p;
+        g->R = res->p;
     }
     g->M = M;
     g->N = N;
@@ -810,11 +805,11 @@ extern "C" void ops_gemm_i8(struct ops *o, int M, int N, int K, struct opnd A, c
 {
     const char *fn = "ops_gemm_i8";
     I8Gemm g;
-    View in[6], out;
+    View in[6], out, res;
     int n = 0;
 
     if (pending() || !product_args(fn, &g, M, N, K, B, sb, bias, C, ctype, R, roff, act, slope,
-                                   &out, in, &n))
+                                   &out, &res, in, &n))
         return;
     if (!i8_view(&in[n], fn, "A", A, M, K) ||
         !view_of(&in[n + 1], fn, "the scales of A", sa, 0, M, 1, M, 4) ||
@@ -847,12 +842,12 @@ extern "C" void ops_linear_i8(struct ops *o, int rows, int in, int out, struct o
 {
     const char *fn = "ops_linear_i8";
     I8Gemm g;
-    View v[6], y, ws;
+    View v[6], y, res, ws;
     int n = 0;
 
     if (pending() || !type_ok(fn, xtype) ||
-        !product_args(fn, &g, rows, out, in, W, sw, bias, Y, ytype, R, roff, act, slope, &y, v,
-                      &n) ||
+        !product_args(fn, &g, rows, out, in, W, sw, bias, Y, ytype, R, roff, act, slope, &y,
+                      &res, v, &n) ||
         !view_of(&v[n], fn, "X", X.buf, X.off, X.ld, rows, in, type_size(xtype)))
         return;
     const View x = v[n++];
@@ -866,7 +861,7 @@ extern "C" void ops_linear_i8(struct ops *o, int rows, int in, int out, struct o
             fail("%s: the work buffer is not 16-byte aligned", fn);
             return;
         }
-        if (!apart(fn, ws, v, n) || !apart(fn, y, &ws, 1))
+        if (!apart(fn, ws, v, n) || !apart(fn, y, &ws, 1) || !apart(fn, ws, &res, 1))
             return;
     }
     OnDevice dev(o->ocl);

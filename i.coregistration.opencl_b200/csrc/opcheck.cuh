@@ -132,7 +132,9 @@ inline int sms_of(const struct ocl_backend *ocl) { return ocl->sm_count > 0 ? oc
 
 // Launches a kernel whose blocks may start while the stream's previous kernel
 // ends (programmatic stream serialization): every thread of it calls
-// after_previous() before its first access to global memory.
+// after_previous() before its first access to global memory, and reads none
+// through the read-only cache, as the previous kernel may have written it
+// since this one started.
 template <typename... P, typename... A>
 bool launch_chained(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem,
                     cudaStream_t st, const A &...args)

@@ -177,7 +177,7 @@ __device__ __forceinline__ bool tile_out(const Params &p, const CUtensorMap *tma
     const TC *R = (const TC *)g.R;
     m0 += 32 * q;
     const int row = m0 + lane;
-    const float sa = row < g.M ? __ldg(g.sa + row) : 0.0f;
+    const float sa = row < g.M ? g.sa[row] : 0.0f;
     constexpr int STEP = COLS * (EPI_WARPS / 4);
     // The residual's blocks come as the output's leave: 64-byte row segments by
     // four lanes each, through the staging block, the first while the

@@ -101,6 +101,9 @@ SHAPES = [
     (4, 9001, 204, 34, (0, 204, 0), (0, 204, 0)),
     (1, 40009, 63, 7, (0, 63, 0), (0, 63, 0)),
     (3, 5, 21, 7, (0, 21, 0), (0, 21, 0)),
+    # Odd channel counts too wide for whole vectors; groups wider than a block.
+    (1, 50, 1003, 17, (0, 1003, 0), (0, 1003, 0)),
+    (2, 9, 9000, 2, (0, 9000, 0), (0, 9000, 0)),
 ]
 
 

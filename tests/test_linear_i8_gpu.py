@@ -202,7 +202,7 @@ def test_gemm_activations_residual(dev, shape, kind, t):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M", [1, 20, 140])
+@pytest.mark.parametrize("M", [1, 2, 3, 12, 20, 140])
 def test_gemm_largest_sums(dev, M):
     """The deepest product of the largest values: 2^31 - 2^14, exact; and K = 0."""
     N, K = 40, coreg.I8_MAX_K

@@ -143,6 +143,7 @@ def test_linear_refusals(h):
     h.refuses("work buffer is not 16-byte", f, *args(work=h.buf(4096, 8)))
     h.refuses("overlaps", f, *args(work=X))
     h.refuses("overlaps", f, *args(work=Y))
+    h.refuses("overlaps", f, *args(work=wk, r=wk))
     h.refuses("overlaps", f, *args(y=M(X, 8)))
     h.runs_nothing(f, *args(m=0, work=None))
     h.runs_nothing(f, *args(n=0, work=None))
