@@ -278,6 +278,14 @@ __device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias)
     return fmaf(__int2float_rn(acc) * sa, sb, bias);
 }
 
+// The activation of a value whose neighbouring column the neighbouring lane has (0
+// behind the last): by the pair, as the tensor-core kernels take it.
+__device__ __forceinline__ float act_beside(float v, int act, float slope)
+{
+    const float other = __shfl_xor_sync(3u << (threadIdx.x % 32 & ~1u), v, 1);
+    return act2_any(make_float2(v, other), act, slope).x;
+}
+
 // Products of depth 0: act(bias) + R.
 template <typename TC>
 __global__ void __launch_bounds__(256)
@@ -287,8 +295,10 @@ i8_empty_k(const I8Gemm g)
     const long n = (long)g.M * g.N;
     for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long)gridDim.x * 256) {
         const long m = e / g.N, c = e - m * g.N, at = m * g.ldc + c;
-        float v = act_any(scaled(0, g.sa[m], g.sb[c], g.bias ? g.bias[c] : 0.0f),
-                          g.act, g.slope);
+        auto value = [&](long j) {
+            return j < g.N ? scaled(0, g.sa[m], g.sb[j], g.bias ? g.bias[j] : 0.0f) : 0.0f;
+        };
+        float v = act2_any(make_float2(value(c), value(c ^ 1)), g.act, g.slope).x;
         if (g.R)
             v += ldf((const TC *)g.R + at);
         stf((TC *)g.C + at, v);
@@ -404,22 +414,22 @@ __device__ void quant_tokens(const Tokens &x, int M, int K, int8_t *q, float *s,
     __syncthreads();
 }
 
-// NT: groups of 8 tokens. TX: the type of tokens that come unquantised (the
+// TX: the type of tokens that come unquantised (the
 // struct x; then g.A and g.sa are not used), or void.
-template <int NT, typename TC, typename TX>
+template <typename TC, typename TX>
 __global__ void __launch_bounds__(32 * FEW_WARPS)
 i8_few_k(const I8Gemm g, const Tokens x, int split)
 {
     constexpr bool FLOATS = !std::is_same<TX, void>::value;
     constexpr int THREADS = 32 * FEW_WARPS;
-    __shared__ int part[FEW_WARPS][FEW_CH][8 * NT + 1];
-    __shared__ float scale[8 * NT];
-    __shared__ uint32_t amax[8 * NT];
+    __shared__ int part[FEW_WARPS][FEW_CH][8 + 1];
+    __shared__ float scale[8];
+    __shared__ uint32_t amax[8];
     extern __shared__ __align__(16) int8_t tok[];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int channels = FEW_WARPS / split * FEW_CH, c0 = blockIdx.x * channels;
     const int n0 = c0 + warp / split * FEW_CH, r = lane / 4, kk = 16 * (lane % 4);
-    if (FLOATS && threadIdx.x < 8 * NT)
+    if (FLOATS && threadIdx.x < 8)
         amax[threadIdx.x] = 0;
     after_previous();
     const int8_t *w0 = g.B + (long)min(n0 + r, g.N - 1) * g.ldb;
@@ -446,22 +456,18 @@ i8_few_k(const I8Gemm g, const Tokens x, int split)
     else if (threadIdx.x < g.M) {
         scale[threadIdx.x] = g.sa[threadIdx.x];
     }
-    int sum[NT][4] = {};
+    int sum[4] = {};
     for (; k - kk < g.K; k += U * step) {
-        float d[NT][4] = {};
+        float d[4] = {};
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            uint4 v[NT];
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const int m = 8 * t + r, at = k + u * step;
-                v[t] = make_uint4(0, 0, 0, 0);
-                if (m < g.M) {
-                    if (!FLOATS)
-                        v[t] = load16(g.A + (long)m * g.lda, at, g.K);
-                    else if (at < g.K)
-                        v[t] = *(const uint4 *)(tok + m * x.pitch + at);
-                }
+            uint4 v = make_uint4(0, 0, 0, 0);
+            const int at = k + u * step;
+            if (r < g.M) {
+                if (!FLOATS)
+                    v = load16(g.A + (long)r * g.lda, at, g.K);
+                else if (at < g.K)
+                    v = *(const uint4 *)(tok + r * x.pitch + at);
             }
             const uint32_t wa[4] = {a[u].x, a[u].y, a[u].z, a[u].w};
             const uint32_t wb[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
@@ -470,12 +476,9 @@ i8_few_k(const I8Gemm g, const Tokens x, int split)
                 uint32_t a0, a1, a2, a3;
                 halves(wa[i], a0, a2);
                 halves(wb[i], a1, a3);
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    uint32_t b0, b1;
-                    halves(i == 0 ? v[t].x : i == 1 ? v[t].y : i == 2 ? v[t].z : v[t].w, b0, b1);
-                    mma_f16(d[t], a0, a1, a2, a3, b0, b1);
-                }
+                uint32_t b0, b1;
+                halves(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w, b0, b1);
+                mma_f16(d, a0, a1, a2, a3, b0, b1);
             }
         }
 #pragma unroll
@@ -485,24 +488,20 @@ i8_few_k(const I8Gemm g, const Tokens x, int split)
         }
         // U steps are 256 of depth.
 #pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                sum[t][i] += __float2int_rn(d[t][i]);
+        for (int i = 0; i < 4; i++)
+            sum[i] += __float2int_rn(d[i]);
     }
 #pragma unroll
-    for (int t = 0; t < NT; t++)
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            part[warp][r + 8 * (i / 2)][8 * t + 2 * (lane % 4) + i % 2] = sum[t][i];
+    for (int i = 0; i < 4; i++)
+        part[warp][r + 8 * (i / 2)][2 * (lane % 4) + i % 2] = sum[i];
     __syncthreads();
-    if (!out)
-        return;
     for (int m = m0; m < g.M; m += THREADS / channels) {
         int s = 0;
-        for (int i = 0; i < split; i++)
+        for (int i = 0; i < split && out; i++)
             s += part[c / FEW_CH * split + i][c % FEW_CH][m];
-        float v = act_any(scaled(s, scale[m], sb, bias), g.act, g.slope);
+        float v = act_beside(scaled(s, scale[m], sb, bias), g.act, g.slope);
+        if (!out)
+            continue;
         const long at = (long)m * g.ldc + c0 + c;
         if (g.R)
             v += ldf((const TC *)g.R + at);
@@ -590,13 +589,13 @@ i8_dot_k(const I8Gemm g, const Tokens x, int split)
                 part[warp][r][m] = s;
         }
     __syncthreads();
-    if (!out)
-        return;
     for (int m = m0; m < g.M; m += THREADS / channels) {
         int s = 0;
-        for (int i = 0; i < split; i++)
+        for (int i = 0; i < split && out; i++)
             s += part[c / DOT_ROWS * split + i][c % DOT_ROWS][m];
-        float v = act_any(scaled(s, scale[m], sb, bias), g.act, g.slope);
+        float v = act_beside(scaled(s, scale[m], sb, bias), g.act, g.slope);
+        if (!out)
+            continue;
         const long at = (long)m * g.ldc + c0 + c;
         if (g.R)
             v += ldf((const TC *)g.R + at);
@@ -623,30 +622,34 @@ void few(cudaStream_t st, const I8Gemm &g, const Tokens &x, int sms)
         launch_chained(i8_dot_k<1, TC, TX>, grid, T, smem, st, g, x, split);
     else if (dot)
         launch_chained(i8_dot_k<2, TC, TX>, grid, T, smem, st, g, x, split);
-    else if (g.M <= 8)
-        launch_chained(i8_few_k<1, TC, TX>, grid, T, smem, st, g, x, split);
     else
-        launch_chained(i8_few_k<2, TC, TX>, grid, T, smem, st, g, x, split);
+        launch_chained(i8_few_k<TC, TX>, grid, T, smem, st, g, x, split);
 }
 
-// Tokens that the streaming kernels take: up to two the dot products always;
-// up to 16 where the layer is no wider than the tensor cores' tiles fill the
-// device with (they take about 0.3 us per 128 bytes of depth at any width, these
-// 0.4 us per million weights up to 8 tokens and 0.6 up to 16: 8 tokens, 8192 x
-// 8192 32 against 21 us, 1024 x 1024 4.6 against 5.7).
-constexpr int FEW_ROWS = 16;
-bool streams(int M, int N)
+// Products that the streaming kernels take: small ones, which on the tcgen05
+// cores take the same time or more. Both sides in us, calls among others (M x N
+// x K): 1 x 4096 x 2048 5.3 and 5.4, 1 x 8192 x 1500 8.4 and 5.4; 2 x 1024 x
+// 4096 5.2 and 5.4, 2 x 4096 x 2048 6.2 and 5.4; 8 x 4096 x 1024 4.9 and 5.1,
+// 8 x 8192 x 1024 7.9 and 5.4; 8 x 1024 x 4096, where a warp's chain over the
+// depth is long, 7.5 and 5.4.
+constexpr int FEW_ROWS = 8;
+bool streams(int M, int N, int K)
 {
-    return M <= DOT_TOKENS || (M <= 8 && N <= 6144) || (M <= FEW_ROWS && N <= 4096);
+    const long weights = (long)N * K;
+    return M == 1   ? weights <= 8 << 20
+           : M == 2 ? weights <= 4 << 20
+                    : M <= FEW_ROWS && weights <= 4 << 20 && K <= 2048;
 }
 
 // Rows that ops_linear_i8 quantises within the product: every block does it
-// again, so that it pays for few values only (16 x 1024 to 4096 channels 8.8 us
-// against 8.7 in two launches, 8 x 1024 6.4, one token 4.7 against 10).
-constexpr int FUSED_VALUES = 16384;
+// again, so that it pays for few values only (us in one launch and in two,
+// rows x out x in: 1 x 4096 x 1024 4.7 and 6.7, 8 x 1024 x 512 6.0 and 6.6, 4 x
+// 4096 x 1024 6.2 and 6.8; 8 x 8192 x 1024 11.8 and 7.0, 1 x 4096 x 4096 8.7 and
+// 7.9).
+constexpr int FUSED_VALUES = 4096, FUSED_IN = 2048;
 bool fused(int rows, int in)
 {
-    return rows <= FEW_ROWS && (long)rows * in <= FUSED_VALUES;
+    return rows <= FEW_ROWS && in <= FUSED_IN && (long)rows * in <= FUSED_VALUES;
 }
 
 void linear_fused(const struct ocl_backend *ocl, const I8Gemm &g, const View &X, int xtype)
@@ -667,7 +670,7 @@ void linear_fused(const struct ocl_backend *ocl, const I8Gemm &g, const View &X,
 void gemm_i8(const struct ocl_backend *ocl, const I8Gemm &g)
 {
     cudaStream_t st = stream_of(ocl);
-    if (streams(g.M, g.N)) {
+    if (streams(g.M, g.N, g.K)) {
         const Tokens none = {nullptr, 0, 0};
         if (g.c_bf16)
             few<__nv_bfloat16, void>(st, g, none, sms_of(ocl));

@@ -136,20 +136,31 @@ inline int sms_of(const struct ocl_backend *ocl) { return ocl->sm_count > 0 ? oc
 // through the read-only cache, as the previous kernel may have written it
 // since this one started.
 template <typename... P, typename... A>
-bool launch_chained(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem,
-                    cudaStream_t st, const A &...args)
+bool launch_clusters(void (*kernel)(P...), dim3 grid, unsigned cluster, unsigned threads,
+                     size_t smem, cudaStream_t st, const A &...args)
 {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster ? 2 : 1;
     return cuda_ok(cudaLaunchKernelEx(&cfg, kernel, P(args)...), "kernel launch");
+}
+
+// The same without clusters, or with those of the kernel's own attribute.
+template <typename... P, typename... A>
+bool launch_chained(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem,
+                    cudaStream_t st, const A &...args)
+{
+    return launch_clusters(kernel, grid, 0, threads, smem, st, args...);
 }
 
 }  // namespace coreg
@@ -199,12 +210,14 @@ __device__ __forceinline__ float rcp_fast(float x)
 // unit takes 8 cycles an instruction and warp, and bounds these. Exponents
 // are cut off at 60, where the quotient is below 1e-18 of x, so that the
 // product of the two divisors stays in range. Relative error below 4e-7 for
-// exact z.
+// exact z. A value's last bit depends on its partner, so that kernels with equal
+// results take the same partners; the products are never contracted with what
+// a caller adds, for the same reason.
 __device__ __forceinline__ float2 over_one_plus_exp2(float2 x, float2 z)
 {
     const float a = 1.0f + exp2_fast(fminf(z.x, 60.0f)), b = 1.0f + exp2_fast(fminf(z.y, 60.0f));
     const float r = rcp_fast(a * b);
-    return make_float2(x.x * (b * r), x.y * (a * r));
+    return make_float2(__fmul_rn(x.x, b * r), __fmul_rn(x.y, a * r));
 }
 
 // Exact GELU, x Phi(x), of two values, as x / (1 + 2^(x Q(x^2))): log2(Phi(-x) /
@@ -248,7 +261,8 @@ __device__ __forceinline__ float2 act2(float2 v, float slope)
     if (ACT == ACT_RELU)
         return make_float2(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f));
     if (ACT == ACT_LEAKY)
-        return make_float2(v.x >= 0.0f ? v.x : slope * v.x, v.y >= 0.0f ? v.y : slope * v.y);
+        return make_float2(v.x >= 0.0f ? v.x : __fmul_rn(slope, v.x),
+                           v.y >= 0.0f ? v.y : __fmul_rn(slope, v.y));
     if (ACT == ACT_GELU_TANH) {
         // 2^(-2 y / ln 2): -2 sqrt(2 / pi) / ln 2 and 0.044715 of that.
         const float2 u = fma2(v, v, pair(0.0f));
@@ -267,19 +281,24 @@ __device__ __forceinline__ float act1(float v, float slope)
 }
 
 // The same with the activation known at run time only.
-__device__ __forceinline__ float act_any(float v, int act, float slope)
+__device__ __forceinline__ float2 act2_any(float2 v, int act, float slope)
 {
     switch (act) {
     case ACT_GELU:
-        return act1<ACT_GELU>(v, slope);
+        return act2<ACT_GELU>(v, slope);
     case ACT_RELU:
-        return act1<ACT_RELU>(v, slope);
+        return act2<ACT_RELU>(v, slope);
     case ACT_LEAKY:
-        return act1<ACT_LEAKY>(v, slope);
+        return act2<ACT_LEAKY>(v, slope);
     case ACT_GELU_TANH:
-        return act1<ACT_GELU_TANH>(v, slope);
+        return act2<ACT_GELU_TANH>(v, slope);
     case ACT_SILU:
-        return act1<ACT_SILU>(v, slope);
+        return act2<ACT_SILU>(v, slope);
     }
     return v;
+}
+
+__device__ __forceinline__ float act_any(float v, int act, float slope)
+{
+    return act2_any(make_float2(v, 0.0f), act, slope).x;
 }

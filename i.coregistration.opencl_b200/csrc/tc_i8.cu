@@ -16,7 +16,8 @@
 //               the matrix's edge); rows that no tensor map can describe go
 //               out through the same block.
 // Bytes of a row behind K, rows behind M and N: outside the tensor maps,
-// which read them as zeros. Every mbarrier wait is bounded (tc_common.cuh).
+// which read them as zeros (of fewer rows than a tile's, see box_rows). Every
+// mbarrier wait is bounded (tc_common.cuh).
 
 #include <type_traits>
 
@@ -45,8 +46,18 @@ struct Params {
     // so that the last columns go out without the tensor map.
     int clean;
     int al;   // sb and bias are 16-byte aligned
-    int al_r; // rows of R are
+    int al_r; // rows of R are (in split depths: 1, and 2 where those of C are)
 };
+
+// Rows of A that a load brings, of M: a tile's, or where there are fewer only those,
+// in eights. Rows outside the tensor map are read as zeros, but each costs more than
+// a row inside it (8 tokens as 128 rows x 8192 x 1500 11 us, as 8 rows 5.6). What
+// a stage holds behind them reaches only sums that nothing reads. (The
+// last tile of many with a box of its own: no gain.)
+__host__ __device__ __forceinline__ int box_rows(int M, int tile)
+{
+    return M < tile ? (M + 7) / 8 * 8 : tile;
+}
 
 template <int BN>
 constexpr int stages() { return BN == 256 ? 4 : BN == 128 ? 6 : 8; }
@@ -98,6 +109,59 @@ __device__ __forceinline__ void load_cols(float v[16], const float *p, int col, 
 #pragma unroll
     for (int j = 0; j < 16; j++)
         v[j] = col + j < n ? p[j] : 0.0f;
+}
+
+// Four neighbours of p, zero behind n and where p is NULL; al: 16-byte
+// aligned as float (8 as bfloat16).
+__device__ __forceinline__ void load_quad(float v[4], const float *p, int n, bool al)
+{
+    if (p && al && n >= 4) {
+        const float4 x = *(const float4 *)p;
+        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        v[j] = p && j < n ? p[j] : 0.0f;
+}
+
+__device__ __forceinline__ void load_quad(float v[4], const __nv_bfloat16 *p, int n, bool al)
+{
+    if (p && al && n >= 4) {
+        const uint2 x = *(const uint2 *)p;
+        v[0] = __uint_as_float(x.x << 16), v[1] = __uint_as_float(x.x & 0xffff0000u);
+        v[2] = __uint_as_float(x.y << 16), v[3] = __uint_as_float(x.y & 0xffff0000u);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        v[j] = p && j < n ? ldf(p + j) : 0.0f;
+}
+
+__device__ __forceinline__ void store_quad(float *p, const float v[4], int n, bool al)
+{
+    if (al && n >= 4) {
+        *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (j < n)
+            p[j] = v[j];
+}
+
+__device__ __forceinline__ void store_quad(__nv_bfloat16 *p, const float v[4], int n, bool al)
+{
+    if (al && n >= 4) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]),
+                             b = __floats2bfloat162_rn(v[2], v[3]);
+        *(uint2 *)p = make_uint2(*(const uint32_t *)&a, *(const uint32_t *)&b);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (j < n)
+            stf(p + j, v[j]);
 }
 
 // Address of 16-byte chunk c of row l of an output block, in its tensor map's
@@ -279,7 +343,9 @@ __device__ __forceinline__ bool tile_out(const Params &p, const CUtensorMap *tma
     return true;
 }
 
-template <int BN, int ACT, typename TC>
+// FEW: fewer rows than a tile's. (Kernels of their own: the box's bytes as a
+// variable cost the others 0.1 us a call.)
+template <int BN, int ACT, bool FEW, typename TC>
 __global__ void __launch_bounds__(NTHREADS, 1)
 tc_i8_k(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
         const __grid_constant__ CUtensorMap tma_c, const Params p)
@@ -325,7 +391,7 @@ tc_i8_k(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUten
                         ok = false;
                         break;
                     }
-                    mbar_expect_tx(&s.full[st], (BM + BN) * BK);
+                    mbar_expect_tx(&s.full[st], ((FEW ? box_rows(g.M, BM) : BM) + BN) * BK);
                     tma_load_2d(s.a[st], &tma_a, &s.full[st], kb * BK, m0);
                     tma_load_2d(s.b[st], &tma_b, &s.full[st], kb * BK, n0);
                 }
@@ -483,10 +549,20 @@ __device__ __forceinline__ bool pair_wait(uint64_t *b, uint32_t parity, int code
     }
 }
 
+__device__ __forceinline__ void cluster_arrive()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void cluster_wait()
+{
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 __device__ __forceinline__ void cluster_sync()
 {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
-                     : "memory");
+    cluster_arrive();
+    cluster_wait();
 }
 
 template <int ACT, typename TC>
@@ -621,6 +697,201 @@ tc_i8_pair_k(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ 
     }
 }
 
+// ------------------------------------------------------------ split depth
+//
+// One 128 x BN tile by a cluster of S CTAs, each over a part of the depth: for
+// deep products of few tiles, in which a CTA's chain of stages (some 600
+// cycles per 128 bytes of depth) is the time (us, M x N x K: 33 x 1024 x 8192
+// 20.4 -> 6.6, 128 x 4096 x 4096 12.5 -> 8.5, 256 x 1024 x 4096 12.4 -> 6.3, 8 x
+// 8192 x 8192 32 -> 15, 4.5 TB/s of weights, the call's some 4 us included;
+// tiles 256 wide for few rows took the same). A CTA hands its sums of the r-th
+// S-th of the columns to the cluster's CTA r, through that one's shared
+// memory, and finishes its own columns from all S parts. The sums are
+// integers: the split changes no result.
+// ROWS: rows of A that a stage holds. For up to 32 tokens it keeps only those, in
+// twice the stages: the products read 128 rows all the same, the others from
+// the stages behind (b is behind a, and larger), into sums that nothing reads
+// (16 x 8192 x 8192 17.0 us with 128 rows and four stages, 15.6).
+template <int BN, int ROWS>
+struct SplitSmem {
+    static constexpr int ST = ROWS == 32 ? 8 : BN == 128 ? 4 : 6;
+    // Four columns of the rows, 16 bytes a row (32 bytes more keep the finishing
+    // reads, neighbouring quads of columns first, off each other's banks).
+    static constexpr int QUAD = ROWS * 16 + 32;
+    alignas(1024) unsigned char a[ST][ROWS * BK];
+    alignas(1024) unsigned char b[ST][BN * BK];
+    // [CTA they come from][quad of this one's columns][row].
+    alignas(16) unsigned char part[BN / 4 * QUAD];
+    uint64_t full[ST], empty[ST], acc_full;
+    uint32_t tmem;
+};
+
+// 16 bytes into the same place of the cluster's CTA r.
+__device__ __forceinline__ void store_to(uint32_t at, int r, const float *v)
+{
+    uint32_t to;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(at), "r"(r));
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(v[0]), "f"(v[1]),
+                 "f"(v[2]), "f"(v[3])
+                 : "memory");
+}
+
+template <int BN, int ROWS, int S, typename TC>
+__global__ void __launch_bounds__(NTHREADS, 1)
+tc_i8_split_k(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
+              const Params p)
+{
+    using Smem = SplitSmem<BN, ROWS>;
+    constexpr int ST = Smem::ST, QUAD = Smem::QUAD, THREADS = 32 * EPI_WARPS;
+    constexpr int NQ = BN / 4 / S;                               // quads of a CTA's columns
+    constexpr int ITEMS = (NQ * ROWS + THREADS - 1) / THREADS;   // of a thread: a row of a quad
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    Smem &s =
+        *reinterpret_cast<Smem *>(smem_raw + ((1024u - (su32(smem_raw) & 1023u)) & 1023u));
+    const I8Gemm &g = p.g;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int rank = (int)cta_rank(), tile = blockIdx.x / S;
+    const int nk = (g.K + BK - 1) / BK;
+    const int tiles_m = (g.M + BM - 1) / BM;
+    const int m0 = tile % tiles_m * BM, n0 = tile / tiles_m * BN;
+    // This CTA's depth (nk >= S).
+    const int kb0 = (int)((long)nk * rank / S), kb1 = (int)((long)nk * (rank + 1) / S);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < ST; i++) {
+            mbar_init(&s.full[i], 1);
+            mbar_init(&s.empty[i], 1);
+        }
+        mbar_init(&s.acc_full, 1);
+        mbar_fence_init();
+    }
+    if (warp == 1)
+        tmem_alloc(&s.tmem, BN);
+    after_previous();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    // Every CTA of the cluster has started: its shared memory may be written.
+    // (Waited for by the epilogue only.)
+    cluster_arrive();
+    const uint32_t tmem = s.tmem;
+    // Scales, bias and residual of the thread's items, fetched meanwhile.
+    float sa[ITEMS], sb[ITEMS][4], bias[ITEMS][4], res[ITEMS][4];
+    bool live[ITEMS];
+    const int me = threadIdx.x - 64;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int kb = kb0; kb < kb1; kb++) {
+                const int it = kb - kb0, st = it % ST;
+                if (it >= ST && !mbar_wait(&s.empty[st], ((it / ST) - 1) & 1, 81))
+                    break;
+                mbar_expect_tx(&s.full[st], (box_rows(g.M, ROWS) + BN) * BK);
+                tma_load_2d(s.a[st], &tma_a, &s.full[st], kb * BK, m0);
+                tma_load_2d(s.b[st], &tma_b, &s.full[st], kb * BK, n0);
+            }
+        }
+        __syncwarp();
+        cluster_wait();
+    }
+    else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_i8(BM, BN);
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; kb++) {
+                const int it = kb - kb0, st = it % ST;
+                if (!mbar_wait(&s.full[st], (it / ST) & 1, 82)) {
+                    ok = false;
+                    break;
+                }
+                const uint64_t da = sw128_desc(su32(s.a[st])), db = sw128_desc(su32(s.b[st]));
+#pragma unroll
+                for (int k = 0; k < BK / 32; k++)
+                    mma_i8(tmem, da + 2 * k, db + 2 * k, idesc, (it > 0 || k > 0) ? 1u : 0u);
+                mma_commit(&s.empty[st]);
+            }
+            if (ok)
+                mma_commit(&s.acc_full);
+        }
+        __syncwarp();
+        cluster_wait();
+    }
+    else {
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) {
+            const int id = me + THREADS * i, row = m0 + id / NQ;
+            const int col = n0 + (rank * NQ + id % NQ) * 4;
+            live[i] = id < NQ * ROWS && row < g.M && col < g.N;
+            if (!live[i])
+                continue;
+            sa[i] = g.sa[row];
+            load_quad(sb[i], g.sb + col, g.N - col, p.al);
+            load_quad(bias[i], g.bias ? g.bias + col : nullptr, g.N - col, p.al);
+            load_quad(res[i], g.R ? (const TC *)g.R + (long)row * g.ldc + col : nullptr,
+                      g.N - col, p.al_r & 1);
+        }
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(&s.acc_full, 0, 83));
+        cluster_wait();
+        const int q = warp % 4, r = 32 * q + lane;
+        if (ok && m0 + 32 * q < g.M) {
+            fence_after();
+            const uint32_t acc = tmem + ((uint32_t)(32 * q) << 16);
+            for (int c0 = 16 * ((warp - 2) / 4); c0 < BN; c0 += 16 * (EPI_WARPS / 4)) {
+                float v[16];
+                tmem_ld16(acc + c0, v);
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int quad = c0 / 4 + k;
+                    store_to(su32(s.part + (rank * NQ + quad % NQ) * QUAD + r * 16), quad / NQ,
+                             v + 4 * k);
+                }
+            }
+            fence_before();
+        }
+    }
+    // The parts have arrived.
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    if (warp >= 2) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) {
+            if (!live[i])
+                continue;
+            const int id = me + THREADS * i, quad = id % NQ, r = id / NQ;
+            const int row = m0 + r, col = n0 + (rank * NQ + quad) * 4;
+            int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll
+            for (int from = 0; from < S; from++) {
+                const int4 x = *(const int4 *)(s.part + (from * NQ + quad) * QUAD + r * 16);
+                sum.x += x.x;
+                sum.y += x.y;
+                sum.z += x.z;
+                sum.w += x.w;
+            }
+            // The token's scale first (see scaled() in linear_i8.cu).
+            const float y[4] = {__int2float_rn(sum.x) * sa[i], __int2float_rn(sum.y) * sa[i],
+                                __int2float_rn(sum.z) * sa[i], __int2float_rn(sum.w) * sa[i]};
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+                const float2 x = act2_any(make_float2(fmaf(y[j], sb[i][j], bias[i][j]),
+                                                      fmaf(y[j + 1], sb[i][j + 1], bias[i][j + 1])),
+                                          g.act, g.slope);
+                v[j] = g.R ? x.x + res[i][j] : x.x;
+                v[j + 1] = g.R ? x.y + res[i][j + 1] : x.y;
+            }
+            store_quad((TC *)g.C + (long)row * g.ldc + col, v, g.N - col, p.al_r & 2);
+        }
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        fence_after();
+        tmem_dealloc(tmem, BN);
+    }
+}
+
 // The kernel of an activation.
 template <typename F>
 bool with_act(int act, F f)
@@ -653,7 +924,7 @@ bool launch(cudaStream_t st, const I8Gemm &g, int sms)
     CUtensorMap ma, mb, mc = {};
     Params p;
     p.g = g;
-    if (!make_map_rows(&ma, g.A, 1, g.M, g.K, g.lda, BK, BM, 128) ||
+    if (!make_map_rows(&ma, g.A, 1, g.M, g.K, g.lda, BK, box_rows(g.M, BM), 128) ||
         !make_map_rows(&mb, g.B, 1, g.N, g.K, g.ldb, BK, PAIR ? BN / 2 : BN, 128))
         return false;
     p.tma_out = make_map_rows(&mc, g.C, sizeof(TC), g.M, g.N, g.ldc * (long)sizeof(TC),
@@ -668,51 +939,147 @@ bool launch(cudaStream_t st, const I8Gemm &g, int sms)
     const unsigned grid = (unsigned)(tiles < most ? tiles : most) * (PAIR ? 2 : 1);
     return with_act(g.act, [&](auto act) {
         constexpr int ACT = decltype(act)::value;
-        static unsigned done = 0;
         if constexpr (PAIR) {
+            static unsigned done = 0;
             const size_t smem = sizeof(PairSmem) + 1024;
             if (!smem_opt_in((const void *)tc_i8_pair_k<ACT, TC>, smem, &done))
                 return false;
             launch_chained(tc_i8_pair_k<ACT, TC>, grid, NTHREADS, smem, st, ma, mb, mc, p);
+            return true;
         }
         else {
-            const size_t smem = sizeof(Smem<BN>) + 1024;
-            if (!smem_opt_in((const void *)tc_i8_k<BN, ACT, TC>, smem, &done))
-                return false;
-            launch_chained(tc_i8_k<BN, ACT, TC>, grid, NTHREADS, smem, st, ma, mb, mc, p);
+            auto go = [&](auto kernel, unsigned *done) {
+                const size_t smem = sizeof(Smem<BN>) + 1024;
+                if (!smem_opt_in((const void *)kernel, smem, done))
+                    return false;
+                launch_chained(kernel, grid, NTHREADS, smem, st, ma, mb, mc, p);
+                return true;
+            };
+            static unsigned done[2] = {0, 0};
+            return g.M < BM ? go(tc_i8_k<BN, ACT, true, TC>, &done[1])
+                            : go(tc_i8_k<BN, ACT, false, TC>, &done[0]);
         }
-        return true;
     });
 }
+
+template <int BN, int ROWS, int S, typename TC>
+bool launch_split(cudaStream_t st, const I8Gemm &g)
+{
+    CUtensorMap ma, mb;
+    Params p = {};
+    p.g = g;
+    if (!make_map_rows(&ma, g.A, 1, g.M, g.K, g.lda, BK, box_rows(g.M, ROWS), 128) ||
+        !make_map_rows(&mb, g.B, 1, g.N, g.K, g.ldb, BK, BN, 128))
+        return false;
+    p.al = (((uintptr_t)g.sb | (uintptr_t)g.bias) & 15) == 0;
+    if (g.ldc * (long)sizeof(TC) % 16 == 0)
+        p.al_r = (((uintptr_t)g.R & 15) == 0) | (((uintptr_t)g.C & 15) == 0) << 1;
+    const size_t smem = sizeof(SplitSmem<BN, ROWS>) + 1024;
+    static unsigned done = 0;
+    if (!smem_opt_in((const void *)tc_i8_split_k<BN, ROWS, S, TC>, smem, &done))
+        return false;
+    launch_clusters(tc_i8_split_k<BN, ROWS, S, TC>, (unsigned)(cdiv(g.M, BM) * cdiv(g.N, BN) * S), S,
+                    NTHREADS, smem, st, ma, mb, p);
+    return true;
+}
+
+// Clusters of a split's kernel that run at one time.
+template <int BN, int ROWS, int S, typename TC>
+int split_clusters()
+{
+    static int known = 0;
+    if (!known) {
+        const size_t smem = sizeof(SplitSmem<BN, ROWS>) + 1024;
+        const void *fn = (const void *)tc_i8_split_k<BN, ROWS, S, TC>;
+        static unsigned done = 0;
+        if (!smem_opt_in(fn, smem, &done))
+            return 0;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(S);
+        cfg.blockDim = dim3(NTHREADS);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = S;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            return 0;
+        }
+        known = n;
+    }
+    return known;
+}
+
+template <typename TC>
+struct Choice {
+    const I8Gemm &g;
+    bool (*run)(cudaStream_t, const I8Gemm &, int) = nullptr;
+    double t = 0;
+
+    void offer(double time, bool (*f)(cudaStream_t, const I8Gemm &, int))
+    {
+        if (!run || time < t) {
+            t = time;
+            run = f;
+        }
+    }
+    // One round of clusters only: a second one starts after the first has ended, its
+    // setup and fill unoverlapped (256 x 4096 x 4096 in halves 10.6 us, in
+    // quarters, two rounds, 16.6).
+    template <int BN, int ROWS, int S>
+    void offer_split()
+    {
+        const int nk = cdiv(g.K, BK);
+        if (nk < S || (g.M <= 32) != (ROWS == 32))
+            return;
+        const long tiles = (long)cdiv(g.M, BM) * cdiv(g.N, BN);
+        const double cells = (double)(g.M < BM ? g.M : BM) * BN;
+        const double epi = 1500.0 + 0.39 * cells;
+        const double time = 600.0 * cdiv(nk, S) + 500.0 + (epi > 4400.0 ? epi : 4400.0);
+        if (time < t && tiles <= split_clusters<BN, ROWS, S, TC>())
+            offer(time, [](cudaStream_t st, const I8Gemm &p, int) {
+                return launch_split<BN, ROWS, S, TC>(st, p);
+            });
+    }
+    template <int BN>
+    void offer_whole(int sms)
+    {
+        const long tiles = (long)cdiv(g.M, BM) * cdiv(g.N, BN), rounds = (tiles + sms - 1) / sms;
+        const double main = 600.0 * cdiv(g.K, BK), epi = 1500.0 + 20.0 * BN;
+        offer(rounds * ((main > epi ? main : epi) + 500.0) + epi,
+              BN == 256 && pair_pays(g) ? launch<256, true, TC> : launch<BN, false, TC>);
+    }
+};
 
 template <typename TC>
 bool choose(cudaStream_t st, const I8Gemm &g, int sms)
 {
-    // The width whose tiles take the least time, in cycles: a round of tiles
-    // costs its products or, where that is more, its epilogue, and the last
+    // The tiles that take the least time, in cycles: a round of tiles costs
+    // its products or, where that is more, its epilogue, and the last
     // epilogue overlaps nothing. 128 bytes of depth take about 600 cycles at
     // any width: an MMA reads its 128 rows of A for 128 cycles, in which it
     // multiplies up to 256 columns (25616 x 4096 x 1024 in short runs: 125 us
     // with 256 columns, 144 with 128, 231 with 64; 500 x 500 x 500, where
-    // rounds do not count: 13.5, 10.3 and 8.4).
-    const int widths[3] = {256, 128, 64};
-    int best = 0;
-    double best_t = 0;
-    for (int i = 0; i < 3; i++) {
-        const int bn = widths[i];
-        const long tiles = (long)cdiv(g.M, BM) * cdiv(g.N, bn), rounds = (tiles + sms - 1) / sms;
-        const double main = 600.0 * cdiv(g.K, BK), epi = 1500.0 + 20.0 * bn;
-        const double t = rounds * ((main > epi ? main : epi) + 500.0) + epi;
-        if (i == 0 || t < best_t) {
-            best = i;
-            best_t = t;
-        }
-    }
-    if (best == 0 && pair_pays(g))
-        return launch<256, true, TC>(st, g, sms);
-    return best == 0   ? launch<256, false, TC>(st, g, sms)
-           : best == 1 ? launch<128, false, TC>(st, g, sms)
-                       : launch<64, false, TC>(st, g, sms);
+    // rounds do not count: 13.5, 10.3 and 8.4). A split depth's epilogue is
+    // longer: at 128 x 4096 x 1024 some 3.3 us with 128 columns, 1.7 with 64 and
+    // at 32 rows, against 1.5 unsplit.
+    Choice<TC> c{g};
+    c.template offer_whole<256>(sms);
+    c.template offer_whole<128>(sms);
+    c.template offer_whole<64>(sms);
+    c.template offer_split<128, 32, 2>();
+    c.template offer_split<128, 32, 4>();
+    c.template offer_split<128, 32, 8>();
+    c.template offer_split<64, 128, 2>();
+    c.template offer_split<64, 128, 4>();
+    c.template offer_split<128, 128, 2>();
+    c.template offer_split<128, 128, 4>();
+    c.template offer_split<128, 128, 8>();
+    return c.run(st, g, sms);
 }
 
 }  // namespace

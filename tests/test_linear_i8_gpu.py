@@ -159,6 +159,18 @@ GEMM = [
     (2600, 4352, 2050, 0, 0, 0),
     (5000, 2100, 2064, 0, 1, 4),
     (129, 9000, 4000, 0, 0, 0),
+    # Pairs whose second half has no rows of A, or of B.
+    (2600, 4160, 2048, 0, 0, 0),
+    # Few tiles of a deep product, the depth split; the narrowest and shallowest.
+    (3, 130, 8200, 0, 0, 0),
+    (24, 8192, 520, 0, 0, 0),
+    (32, 900, 4097, 16, 4, 4),
+    (33, 1000, 4096, 0, 0, 0),
+    (10, 1, 700, 0, 0, 0),
+    (48, 2100, 1500, 0, 1, 3),
+    (129, 257, 4097, 0, 2, 2),
+    (256, 300, 3333, 0, 0, 0),
+    (777, 1000, 4100, 0, 0, 0),
 ]
 
 
@@ -183,8 +195,8 @@ def test_gemm(dev, shape, t):
 @pytest.mark.gpu
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("kind", ref.ACTS)
-@pytest.mark.parametrize("shape", [(2, 200, 272), (5, 200, 272), (300, 200, 272), (257, 9000, 2050)],
-                         ids=str)
+@pytest.mark.parametrize("shape", [(2, 200, 272), (5, 200, 272), (300, 200, 272), (257, 9000, 2050),
+                                   (13, 203, 2100), (100, 300, 2100)], ids=str)
 def test_gemm_activations_residual(dev, shape, kind, t):
     """Each activation, without a bias, with a residual of its own and in place."""
     (M, N, K), T = shape, TYPES[t]
@@ -220,6 +232,54 @@ def test_gemm_largest_sums(dev, M):
     dev.lib.ops_gemm_i8(dev.ops_p, M, N, 0, A.opnd, S.handle, B.opnd, S.handle, bias.handle,
                         C.opnd, F32, None, 0, coreg.ACT_RELU, 0.0)
     assert (C.read() == np.maximum(np.arange(N) - 7, 0)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ref.ACTS)
+@pytest.mark.parametrize("N,K", [(201, 4200), (1030, 2048), (4097, 1000), (4160, 2048), (301, 0)])
+def test_gemm_rows_do_not_depend_on_their_number(dev, N, K, kind):
+    """A row's results are the same bits whichever kernel its product takes: by
+    the number of rows the streaming ones, split depths, tiles and pairs."""
+    M = 2600
+    rng = np.random.default_rng(N + K)
+    a, sa, b, sb, bias = operands(rng, M, N, K)
+    A, B = i8_rows(dev, a, extra=16), i8_rows(dev, b, extra=16)
+    SA, SB, BI = dev.upload(sa), dev.upload(sb), dev.upload(bias)
+    R = Rows(dev, M, N, F32, rng.standard_normal((M, N)).astype(np.float32))
+    got = {}
+    for m in (1, 2, 8, 9, 33, 128, 200, 700, M):
+        C = Rows(dev, m, N, F32)
+        dev.lib.ops_gemm_i8(dev.ops_p, m, N, K, A.opnd, SA.handle, B.opnd, SB.handle, BI.handle,
+                            C.opnd, F32, R.handle, 0, ref.ACTS.index(kind), 0.1)
+        got[m] = C.read()
+    for m, c in got.items():
+        assert (c == got[M][:m]).all(), m
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["gelu", "silu"])
+@pytest.mark.parametrize("rows,K,N", [(1, 300, 5001), (1, 9000, 70), (2, 4000, 333),
+                                      (8, 1024, 8191), (8, 1100, 200), (9, 500, 77),
+                                      (40, 2048, 130), (3, 0, 33)])
+def test_linear_is_quant_then_gemm(dev, rows, K, N, kind):
+    """Bit for bit, whether or not the layer is one launch."""
+    rng = np.random.default_rng(rows + K + N)
+    x = tokens(rng, rows, K, F32) if K else np.zeros((rows, 0))
+    qw, sw = ref.quant_i8(rng.standard_normal((N, K))) if K else (np.zeros((N, 0)), np.ones(N))
+    X, W = Rows(dev, rows, K, F32, x, ld=max(K, 1)), i8_rows(dev, qw.astype(np.int8), extra=16)
+    SW, BI = dev.upload(sw), dev.upload(rng.standard_normal(N).astype(np.float32))
+    Q = Rows(dev, rows, K, None, ld=(K + 15) // 16 * 16 + 16)
+    S = dev.upload(np.ones(rows, np.float32))
+    Y, Z = Rows(dev, rows, N, F32), Rows(dev, rows, N, F32)
+    need = dev.lib.ops_linear_i8_bytes(rows, K)
+    work = dev.alloc(need) if need else None
+    act = ref.ACTS.index(kind)
+    dev.lib.ops_linear_i8(dev.ops_p, rows, K, N, X.opnd, F32, W.opnd, SW.handle, BI.handle, Y.opnd,
+                          F32, None, 0, act, 0.0, coreg.handle(work))
+    dev.lib.ops_quant_i8(dev.ops_p, rows, K, X.opnd, F32, Q.opnd, S.handle, 0)
+    dev.lib.ops_gemm_i8(dev.ops_p, rows, N, K, Q.opnd, S.handle, W.opnd, SW.handle, BI.handle,
+                        Z.opnd, F32, None, 0, act, 0.0)
+    assert (Y.read() == Z.read()).all()
 
 
 @pytest.mark.gpu
