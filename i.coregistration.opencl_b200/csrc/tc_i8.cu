@@ -249,19 +249,67 @@ __device__ __forceinline__ bool tile_out(const Params &p, const CUtensorMap *tma
     // L2). Read by one lane per row they took 32 memory lines an
     // instruction, and 14 thousand cycles of a 128 x 256 float tile.
     const bool whole = p.al && n0 + BN <= g.N, by_block = R && p.al_r && n0 + BN <= g.N;
-    uint4 next[4];
+    // Rows that are not 16-byte aligned come value by value, a lane a column (1003
+    // x 3150 x 638 bfloat16 30.5 -> 17.5 us, 2528 x 3250 x 308 float 58 -> 31).
+    uint32_t next[16];
     auto fetch = [&](int c0) {
+        if (by_block) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = m0 + 8 * i + lane / 4;
-            if (r < g.M)
-                next[i] = *((const uint4 *)(R + (long)r * g.ldc + n0 + c0) + lane % 4);
+            for (int i = 0; i < 4; i++) {
+                const int r = m0 + 8 * i + lane / 4;
+                if (r < g.M) {
+                    const uint4 x = *((const uint4 *)(R + (long)r * g.ldc + n0 + c0) + lane % 4);
+                    next[4 * i] = x.x, next[4 * i + 1] = x.y;
+                    next[4 * i + 2] = x.z, next[4 * i + 3] = x.w;
+                }
+            }
+            return;
+        }
+        const int c = n0 + c0 + lane % COLS;
+        const bool in = c < g.N;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            next[i] = 0;
+            if constexpr (sizeof(TC) == 4) {
+                const int r = m0 + 2 * i + lane / 16;
+                if (in && r < g.M)
+                    next[i] = *(const uint32_t *)(R + (long)r * g.ldc + c);
+            }
+            else {
+                const int r = m0 + 2 * i;
+                if (in && r < g.M)
+                    next[i] = *(const uint16_t *)(R + (long)r * g.ldc + c);
+                if (in && r + 1 < g.M)
+                    next[i] |= (uint32_t) * (const uint16_t *)(R + (long)(r + 1) * g.ldc + c) << 16;
+            }
+        }
+    };
+    // What fetch brought, into the staging block.
+    auto put = [&]() {
+        if (by_block) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                *(uint4 *)chunk(cst, 8 * i + lane / 4, lane % 4) =
+                    make_uint4(next[4 * i], next[4 * i + 1], next[4 * i + 2], next[4 * i + 3]);
+            return;
+        }
+        constexpr int E = 16 / (int)sizeof(TC);
+        const int c = lane % COLS;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            if constexpr (sizeof(TC) == 4) {
+                ((uint32_t *)chunk(cst, 2 * i + lane / 16, c / E))[c % E] = next[i];
+            }
+            else {
+                ((uint16_t *)chunk(cst, 2 * i, c / E))[c % E] = (uint16_t)next[i];
+                ((uint16_t *)chunk(cst, 2 * i + 1, c / E))[c % E] = (uint16_t)(next[i] >> 16);
+            }
         }
     };
     if (R && row < g.M)
-        for (int c0 = COLS * part + (by_block ? STEP : 0); c0 < BN && n0 + c0 < g.N; c0 += STEP)
+        for (int c0 = COLS * part + STEP; c0 < BN && n0 + c0 < g.N; c0 += STEP)
             asm volatile("prefetch.global.L2 [%0];" ::"l"(R + (long)row * g.ldc + n0 + c0));
-    if (by_block && COLS * part < BN)
+    if (R && COLS * part < BN && n0 + COLS * part < g.N)
         fetch(COLS * part);
     // Decided per warp: the TMEM loads below are warp-collective.
     if (!__all_sync(0xffffffffu, mbar_wait(full, parity, 63)))
@@ -274,12 +322,10 @@ __device__ __forceinline__ bool tile_out(const Params &p, const CUtensorMap *tma
         if (lane == 0)
             bulk_wait_read<0>();
         __syncwarp();
-        if (by_block) {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                *(uint4 *)chunk(cst, 8 * i + lane / 4, lane % 4) = next[i];
+        if (R) {
+            put();
             __syncwarp();
-            if (c0 + STEP < BN)
+            if (c0 + STEP < BN && n0 + c0 + STEP < g.N)
                 fetch(c0 + STEP);
         }
 #pragma unroll
@@ -309,14 +355,8 @@ __device__ __forceinline__ bool tile_out(const Params &p, const CUtensorMap *tma
                 v[j] = x.x;
                 v[j + 1] = x.y;
             }
-            if (by_block)
+            if (R)
                 add_staged(v, cst, lane, h, (const TC *)nullptr);
-            else if (R && row < g.M) {
-#pragma unroll
-                for (int j = 0; j < 16; j++)
-                    if (at + j < g.N)
-                        v[j] += ldf(R + (long)row * g.ldc + at + j);
-            }
             stage_row(cst, lane, h, v, (TC *)nullptr);
         }
         if (p.tma_out && (col + COLS <= g.N || p.clean)) {
@@ -330,7 +370,8 @@ __device__ __forceinline__ bool tile_out(const Params &p, const CUtensorMap *tma
         }
         __syncwarp();
         // Rows without a tensor map: lane = column, several rows at a time where
-        // they are short.
+        // they are short. (Eight reads ahead of their writes: 19428 x 1298 x 23
+        // bfloat16 76 us against 53.)
         constexpr int E = 16 / (int)sizeof(TC);
         const int c = lane % COLS;
         if (col + c < g.N)
