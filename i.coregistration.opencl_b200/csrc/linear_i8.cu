@@ -89,7 +89,7 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// 16 bytes of a row: V values, or one value where rows are not aligned.
+// 16 bytes of a row: V values; two values or one where rows are not aligned.
 template <typename T, int V>
 struct Piece {
     uint4 w;
@@ -150,6 +150,37 @@ struct Piece {
             else
                 p.w.x >>= 16;
         }
+    }
+};
+
+template <typename T>
+struct Piece<T, 2> {
+    float a, b;
+    __device__ __forceinline__ void load(const T *p)
+    {
+        if constexpr (sizeof(T) == 4) {
+            const float2 x = *(const float2 *)p;
+            a = x.x, b = x.y;
+        }
+        else {
+            const uint32_t x = *(const uint32_t *)p;
+            a = __uint_as_float(x << 16), b = __uint_as_float(x & 0xffff0000u);
+        }
+    }
+    __device__ __forceinline__ uint32_t top() const { return max(magnitude(a), magnitude(b)); }
+    __device__ __forceinline__ void store(int8_t *q, const RowScale &s) const
+    {
+        bool sure = true;
+        uint32_t x = s.guess(a, sure), y = s.guess(b, sure);
+        if (!sure) {
+            if (s.inv > 0.0f) {
+                x = s.settle(x, a), y = s.settle(y, b);
+            }
+            else {
+                x = RowScale::quotient(a, s.s), y = RowScale::quotient(b, s.s);
+            }
+        }
+        *(uint16_t *)q = (uint16_t)__byte_perm(x, y, 0x0040);
     }
 };
 
@@ -232,8 +263,10 @@ quant_k(const T *X, long ldx, long rows, int C, int8_t *Q, long ldq, float *S)
 template <typename T, int V>
 void quant_launch(cudaStream_t st, const View &x, int8_t *q, long ldq, float *s)
 {
-    // A warp per row up to 8 pieces a lane (no barrier of the block), then a
-    // block.
+    // A warp per row up to 8 pieces a lane, or 32 of one or two values (no barrier
+    // of the block), then a block. (us, a block from 8 on and this: 10923 x 397
+    // bfloat16, one value a piece, 16.3 and 7.9, 18142 x 812, two, 28.9 and 17.0.
+    // Two values where rows allow it: 15088 x 3758 bfloat16 105 -> 54.)
     const int pieces = (int)(x.cols / V);
     auto go = [&](auto g, auto np) {
         constexpr int G = decltype(g)::value, NP = decltype(np)::value;
@@ -242,29 +275,45 @@ void quant_launch(cudaStream_t st, const View &x, int8_t *q, long ldq, float *s)
     };
     typedef std::integral_constant<int, 4> four;
     typedef std::integral_constant<int, 8> eight;
+    typedef std::integral_constant<int, 16> sixteen;
+    typedef std::integral_constant<int, 32> thirty_two;
     typedef std::integral_constant<int, 32> warp;
     typedef std::integral_constant<int, 256> block;
     if (pieces <= 32 * 4)
         go(warp(), four());
     else if (pieces <= 32 * 8)
         go(warp(), eight());
+    else if (V <= 2 && pieces <= 32 * 16)
+        go(warp(), sixteen());
+    else if (V <= 2 && pieces <= 32 * 32)
+        go(warp(), thirty_two());
     else if (pieces <= 256 * 4)
         go(block(), four());
+    else if (V <= 2 && pieces > 256 * 8 && pieces <= 256 * 16)
+        go(block(), sixteen());
     else
         go(block(), eight());
 }
 
 void quant_rows(cudaStream_t st, const View &x, int xtype, int8_t *q, long ldq, float *s)
 {
-    const int V = xtype == OPS_BF16 ? 8 : 4;
-    const bool al = ((uintptr_t)x.p & 15) == 0 && (x.rows == 1 || x.ld % V == 0) &&
-                    (uintptr_t)q % V == 0 && (x.rows == 1 || ldq % V == 0);
-    if (xtype == OPS_BF16 && al)
-        quant_launch<__nv_bfloat16, 8>(st, x, q, ldq, s);
-    else if (xtype == OPS_BF16)
-        quant_launch<__nv_bfloat16, 1>(st, x, q, ldq, s);
-    else if (al)
+    const int es = type_size(xtype);
+    auto al = [&](int v) {
+        return (uintptr_t)x.p % (v * es) == 0 && (uintptr_t)q % v == 0 &&
+               (x.rows == 1 || (x.ld % v == 0 && ldq % v == 0));
+    };
+    if (xtype == OPS_BF16) {
+        if (al(8))
+            quant_launch<__nv_bfloat16, 8>(st, x, q, ldq, s);
+        else if (al(2))
+            quant_launch<__nv_bfloat16, 2>(st, x, q, ldq, s);
+        else
+            quant_launch<__nv_bfloat16, 1>(st, x, q, ldq, s);
+    }
+    else if (al(4))
         quant_launch<float, 4>(st, x, q, ldq, s);
+    else if (al(2))
+        quant_launch<float, 2>(st, x, q, ldq, s);
     else
         quant_launch<float, 1>(st, x, q, ldq, s);
 }

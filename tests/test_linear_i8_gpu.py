@@ -49,6 +49,12 @@ QUANT = [
     (2, 20001, 0, 20001, 5, 20003),
     (1601, 96, 0, 96, 0, 96),
     (1, 40000, 0, 40000, 0, 40000),
+    # Rows aligned to two values, or to one: short, and long beyond the registers.
+    (35, 30, 2, 30, 0, 32),
+    (4, 3758, 0, 3758, 0, 3760),
+    (3, 4101, 1, 4101, 0, 4112),
+    (2, 9003, 2, 9006, 2, 9006),
+    (2, 5001, 3, 5003, 1, 5001),
 ]
 
 
@@ -68,7 +74,7 @@ def test_quant_equals(dev, shape, t):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("t", TYPES)
-@pytest.mark.parametrize("C", [5, 48, 1024, 9000])
+@pytest.mark.parametrize("C", [5, 48, 1024, 9000, 26, 4098, 4097])
 def test_quant_edge_rows(dev, C, t):
     """Zeros, infinities, NaN, the type's extremes, denormal rows and exact
     ties (multiples of half a scale)."""
