@@ -19,9 +19,11 @@ namespace {
 // pixels, a thread a fixed vector of channels in every lanes-th of them, so
 // that statistics and coefficients stay in its registers:
 //   1. per thread and channel the mean and M2 (sum of squares about the mean),
-//      from sums about the thread's first value (it has at most some hundred
-//      values, of which that is one: an outlier there costs M2 no more than
-//      their number in rounding steps); the vectors read stay in shared
+//      from sums about the mean of its first eight values; every FOLD vectors
+//      they are joined to a mean and M2 of two floats each and begun again, so
+//      that no chain of roundings is longer than 8 + FOLD / 8 however many
+//      vectors a thread has, and an outlier among the eight costs M2 no more
+//      than some steps of its own square; the vectors read stay in shared
 //      memory as far as they fit;
 //   2. the block's mean and M2 per group from its threads', the team's from
 //      its blocks': weighted means first, then squares about them, so that
@@ -65,6 +67,7 @@ struct GroupNorm {
     int keep, ring;       // vectors a thread keeps, places of the ring (RING or 0)
     int merged;           // neighbouring channels of a thread in one entry
     int simple;           // all of a thread's, and gamma and beta 16-byte aligned
+    int fold;             // entries that a thread folds into: 0 with at most FOLD vectors
     int batch;            // grid teams: images at a time, a team each
     float2 *work;         // grid teams: 2 x batch x groups x team (mean, M2)
 };
@@ -73,6 +76,8 @@ constexpr int MAX_THREADS = 512;
 // Vectors of a thread in flight: 8 x 512 x 16 bytes per multiprocessor cover
 // the memory's latency at its full rate (about 45 KB) with some to spare.
 constexpr int RING = 8;
+// Vectors whose sums are folded together. (Threads of most maps have fewer.)
+constexpr int FOLD = 128;
 constexpr int MAX_TEAM = 160; // blocks of a grid team the work buffer holds
 
 
@@ -174,6 +179,12 @@ __host__ __device__ inline size_t kept_bytes(const GroupNorm &p, int threads, si
     return ((size_t)(p.keep + p.ring) * threads * vec + 15) / 16 * 16;
 }
 
+// Bytes of the block's entries, its (mean, M2) per group and the team's.
+__host__ __device__ inline size_t entry_bytes(const GroupNorm &p)
+{
+    return ((size_t)p.pitch * p.lanes * 8 + (size_t)p.gs * 16 + 15) / 16 * 16;
+}
+
 // Asynchronous copy of 16 bytes into shared memory, by this thread for
 // itself: no barrier, only its own groups.
 __device__ __forceinline__ void fetch16(void *dst, const void *src)
@@ -214,56 +225,169 @@ __device__ __forceinline__ void sums_begin(const GroupNorm &p, const TX *x, cons
     }
 }
 
-// Sums of x - x0 and of its square over a thread's vectors, x0 its first,
-// eight at a time so that no chain of additions is longer than 8 + cnt / 8.
-// Leaves the vectors in shared memory: the first p.keep, and the last RING
-// of the others.
-template <typename TX, int V>
+// The means and M2 of n values each, in the place of their sums s1 and s2 about x0.
+template <int V, typename F>
+__device__ __forceinline__ void settle(const float x0[V], float s1[V], float s2[V], F inv)
+{
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+        const float m = s1[e] * inv(e);
+        s2[e] = fmaxf(s2[e] - s1[e] * m, 0.0f);
+        s1[e] = x0[e] + m;
+    }
+}
+
+// put(k, mean, M2) of K neighbouring of a thread's V channels each, which have
+// n values each.
+template <int V, int K, typename F>
+__device__ __forceinline__ void merge(const float mean[V], const float m2[V], float n, F put)
+{
+#pragma unroll
+    for (int e = 0; e < V; e += K) {
+        float m = mean[e], q = m2[e];
+        if (K > 1) {
+#pragma unroll
+            for (int k = 1; k < K; k++)
+                m += mean[e + k];
+            m *= 1.0f / K;
+            q = 0.0f;
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                const float d = mean[e + k] - m;
+                q += fmaf(n * d, d, m2[e + k]);
+            }
+        }
+        put(e / K, m, q);
+    }
+}
+
+// The same for p.merged neighbouring channels that lie in one group (all of a
+// thread's, four, two or one).
+template <int V, typename F>
+__device__ __forceinline__ void entries(const GroupNorm &p, const float mean[V],
+                                        const float m2[V], float n, F put)
+{
+    if (V > 1 && p.merged == V)
+        merge<V, V>(mean, m2, n, put);
+    else if (V == 8 && p.merged == 4)
+        merge<V, 4>(mean, m2, n, put);
+    else if (V > 2 && p.merged == 2)
+        merge<V, 2>(mean, m2, n, put);
+    else
+        merge<V, 1>(mean, m2, n, put);
+}
+
+// v added to hi + lo, lo the rounding errors of hi.
+__device__ __forceinline__ void add_up(float &hi, float &lo, float v)
+{
+    const float s = hi + v, z = s - hi, e = (hi - (s - z)) + (v - z);
+    lo = fabsf(s) < INFINITY ? lo + e : 0.0f;
+    hi = s;
+}
+
+// (m, q) of some vectors of p.merged channels joined to the (mean, M2) of `before`
+// vectors in an entry, whose rounding errors are at `rest`: two floats hold
+// what one would lose over hundreds of joins (doubles took 4 us of 105 at 132
+// vectors a thread, by their conversions). w: the new vectors' share of all;
+// last: the entry is complete.
+__device__ __forceinline__ void join(const GroupNorm &p, float2 *entry, float2 *rest, int before,
+                                     float m, float q, float w, bool last)
+{
+    float2 hi = make_float2(0.0f, 0.0f), lo = hi;
+    if (before) {
+        hi = *entry;
+        lo = *rest;
+    }
+    const float d = (m - hi.x) - lo.x;
+    add_up(hi.x, lo.x, d * w);
+    add_up(hi.y, lo.y, fmaf(d * d, w * (float)(before * p.merged), q));
+    if (last)
+        hi = make_float2(hi.x + lo.x, hi.y + lo.y);
+    else
+        *rest = lo;
+    *entry = hi;
+}
+
+// Vectors of a thread that are folded when its sums end: whole FOLDs, at
+// least one vector left.
+__device__ __forceinline__ int folded(int cnt) { return cnt > FOLD ? (cnt - 1) / FOLD * FOLD : 0; }
+
+// The sums of a thread's FOLD vectors into its entries from `to` on; `before` are
+// in there.
+template <int V>
+__device__ __forceinline__ void fold_sums(const GroupNorm &p, const float x0[V], float s1[V],
+                                          float s2[V], int before, float2 *to, float2 *rest)
+{
+    const float w = (float)FOLD / (float)(before + FOLD);
+    settle<V>(x0, s1, s2, [](int) { return 1.0f / FOLD; });
+    entries<V>(p, s1, s2, (float)FOLD, [&](int k, float m, float q) {
+        join(p, to + k, rest + k * (int)blockDim.x, before, m, q, w, false);
+    });
+}
+
+// The sums t1 and t2 about x0 as the first of a run: of eight values they are
+// taken on to their mean, about which the following ones are added.
+template <int V>
+__device__ __forceinline__ void begin_sums(float x0[V], float s1[V], float s2[V],
+                                           const float t1[V], const float t2[V], bool eight)
+{
+    const float w = eight ? 0.125f : 0.0f, n = eight ? 8.0f : 0.0f;
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+        const float c = fmaf(w, t1[e], x0[e]), d = c - x0[e];
+        s1[e] = fmaf(-n, d, t1[e]);
+        s2[e] = fmaf(-d, t1[e] + s1[e], t2[e]); // n d = t1 - s1
+        x0[e] = c;
+    }
+}
+
+// Sums of x - x0 and of its square over a thread's vectors (those behind the
+// folded ones), eight at a time so that no chain of additions is longer than
+// 8 + FOLD / 8. Leaves the vectors in shared memory: the first p.keep, and the
+// last RING of the others.
+template <typename TX, int V, bool FOLDED>
 __device__ __forceinline__ void sums(const GroupNorm &p, const TX *x, const Place &at, float x0[V],
-                                     float s1[V], float s2[V], typename Vec<TX, V>::Kept *kept)
+                                     float s1[V], float s2[V], typename Vec<TX, V>::Kept *kept,
+                                     float2 *to, float2 *rest)
 {
     const TX *q = at_row(x, p.ldx, p, at, 0);
     const long step = p.lanes * (p.R * p.ldx);
 #pragma unroll
     for (int e = 0; e < V; e++)
         x0[e] = s1[e] = s2[e] = 0.0f;
-    if constexpr (V == 1) {
-        constexpr int U = 8;
-        for (int i0 = 0; i0 < at.cnt; i0 += U, q += U * step) {
-            Vec<TX, V> r[U];
+    if constexpr (V > 1)
+        q += RING * step;
+    // The sums of the vectors i0 .. i1 - 1 (at most eight); first: about the first.
+    float t1[V], t2[V];
+    auto batch = [&](int i0, int i1, bool first) {
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                if (i0 + u < at.cnt)
+        for (int e = 0; e < V; e++)
+            t1[e] = t2[e] = 0.0f;
+        if constexpr (V == 1) {
+            Vec<TX, V> r[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+                if (i0 + u < i1)
                     r[u].load(q + u * step);
-            if (i0 == 0)
+            q += 8 * step;
+            if (first)
                 x0[0] = r[0].at(0);
-            float t1 = 0.0f, t2 = 0.0f;
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                if (i0 + u < at.cnt) {
+            for (int u = 0; u < 8; u++)
+                if (i0 + u < i1) {
                     if (i0 + u < p.keep)
                         r[u].keep(kept + (i0 + u) * blockDim.x);
                     const float d = r[u].at(0) - x0[0];
-                    t1 += d;
-                    t2 = fmaf(d, d, t2);
+                    t1[0] += d;
+                    t2[0] = fmaf(d, d, t2[0]);
                 }
-            s1[0] += t1;
-            s2[0] += t2;
         }
-    }
-    else {
-        q += RING * step;
-        for (int i0 = 0; i0 < at.cnt; i0 += 8) {
-            float t1[V], t2[V];
-#pragma unroll
-            for (int e = 0; e < V; e++)
-                t1[e] = t2[e] = 0.0f;
-            const int i1 = min(i0 + 8, at.cnt);
+        else {
             for (int i = i0; i < i1; i++, q += step) {
                 fetch_wait<RING - 1>();
                 Vec<TX, V> r;
                 r.back(kept + place_of(p, i));
-                if (i == 0) {
+                if (first && i == i0) {
 #pragma unroll
                     for (int e = 0; e < V; e++)
                         x0[e] = r.at(e);
@@ -279,12 +403,26 @@ __device__ __forceinline__ void sums(const GroupNorm &p, const TX *x, const Plac
                     fetch16(kept + place_of(p, i + RING), q);
                 fetch_commit();
             }
+        }
+    };
+    for (int c0 = 0; c0 < at.cnt; c0 += FOLD) {
+        const int c1 = FOLDED ? min(c0 + FOLD, at.cnt) : at.cnt;
+        batch(c0, min(c0 + 8, c1), true);
+        begin_sums<V>(x0, s1, s2, t1, t2, c1 - c0 >= 8);
+        for (int i0 = c0 + 8; i0 < c1; i0 += 8) {
+            batch(i0, min(i0 + 8, c1), false);
 #pragma unroll
             for (int e = 0; e < V; e++) {
                 s1[e] += t1[e];
                 s2[e] += t2[e];
             }
         }
+        if (!FOLDED)
+            break;
+        if (c1 < at.cnt)
+            fold_sums<V>(p, x0, s1, s2, c0, to, rest);
+    }
+    if constexpr (V > 1) {
         if (at.tail > 0) {
             const TX *t = at_row(x, p.ldx, p, at, at.cnt);
 #pragma unroll
@@ -372,30 +510,6 @@ __device__ __forceinline__ void apply(const GroupNorm &p, const TX *x, TY *y, co
     }
 }
 
-// Entries (mean, M2) of K neighbouring of a thread's V channels each, which
-// have n values each.
-template <int V, int K>
-__device__ __forceinline__ void merge(float2 *to, const float mean[V], const float m2[V], float n)
-{
-#pragma unroll
-    for (int e = 0; e < V; e += K) {
-        float m = mean[e], q = m2[e];
-        if (K > 1) {
-#pragma unroll
-            for (int k = 1; k < K; k++)
-                m += mean[e + k];
-            m *= 1.0f / K;
-            q = 0.0f;
-#pragma unroll
-            for (int k = 0; k < K; k++) {
-                const float d = mean[e + k] - m;
-                q += fmaf(n * d, d, m2[e + k]);
-            }
-        }
-        to[e / K] = make_float2(m, q);
-    }
-}
-
 // How a warp walks a group's entries: lane l takes the columns l % pw, + pw, ...
 // of `cols`, and of each the rows l / pw, + 32 / pw, ... (pw a power of two), so
 // that the loops hold no division. visit(column, row).
@@ -410,8 +524,9 @@ __device__ __forceinline__ void walk(int cols, int lanes, int lane, F visit)
 
 // GRID: all blocks at once (a cooperative launch) in teams of a batch of images,
 // batches one after the other; otherwise a team is a cluster, one per image
-// and slice.
-template <typename TX, typename TY, int V, bool GRID>
+// and slice. FOLDED: threads with more than FOLD vectors. (Within one kernel the
+// code for them cost the others 0.1 to 0.7 us.)
+template <typename TX, typename TY, int V, bool GRID, bool FOLDED>
 __global__ void __launch_bounds__(MAX_THREADS, 1)
 groupnorm_k(const __grid_constant__ GroupNorm p)
 {
@@ -421,6 +536,7 @@ groupnorm_k(const __grid_constant__ GroupNorm p)
     float2 *entry = (float2 *)(smem + kept_bytes(p, blockDim.x, sizeof(*kept)));
     float2 *mine = entry + p.pitch * p.lanes; // the block's (mean, M2) per group
     float2 *team = mine + p.gs;               // the team's (mean, 1 / sigma)
+    float2 *rest = (float2 *)((unsigned char *)entry + entry_bytes(p)) + tid; // (if p.fold)
     // (The blocks of a cluster team are a power of two.)
     const int which = GRID ? (int)blockIdx.x / p.team : 0; // the team's image of a batch
     const int rank = GRID ? (int)blockIdx.x - which * p.team : (int)(blockIdx.x & (p.team - 1));
@@ -495,28 +611,26 @@ groupnorm_k(const __grid_constant__ GroupNorm p)
             }
         {
             float x0[V], s1[V], s2[V];
-            sums<TX, V>(p, x, at, x0, s1, s2, kept);
-            // 2. Entries (mean, M2): of p.merged neighbouring channels that lie in
-            // one group (all of a thread's, four, two or one).
+            float2 *to = entry + row * p.pitch + (at.j0 >> (31 - __clz(p.merged)));
+            sums<TX, V, FOLDED>(p, x, at, x0, s1, s2, kept, to, rest);
+            // 2. The thread's entries (mean, M2).
             if (active) {
-                const float i0 = at.cnt > 0 ? 1.0f / (float)at.cnt : 0.0f,
-                            i1 = at.tail > 0 ? 1.0f / (float)(at.cnt + 1) : 0.0f;
-#pragma unroll
-                for (int e = 0; e < V; e++) {
-                    const float m = s1[e] * (e < at.tail ? i1 : i0);
-                    s2[e] = fmaxf(s2[e] - s1[e] * m, 0.0f);
-                    s1[e] = x0[e] + m;
+                const int before = FOLDED ? folded(at.cnt) : 0, left = at.cnt - before;
+                const float i0 = left > 0 ? 1.0f / (float)left : 0.0f,
+                            i1 = at.tail > 0 ? 1.0f / (float)(left + 1) : 0.0f;
+                settle<V>(x0, s1, s2, [&](int e) { return e < at.tail ? i1 : i0; });
+                if (before == 0)
+                    entries<V>(p, s1, s2, (float)left,
+                               [&](int k, float m, float q) { to[k] = make_float2(m, q); });
+                else {
+                    // (With a tail a thread's entries are single channels.)
+                    const float w0 = (float)left / (float)at.cnt,
+                                w1 = (float)(left + 1) / (float)(at.cnt + 1);
+                    entries<V>(p, s1, s2, (float)left, [&](int k, float m, float q) {
+                        join(p, to + k, rest + k * (int)blockDim.x, before, m, q,
+                             k < at.tail ? w1 : w0, true);
+                    });
                 }
-                float2 *to = entry + row * p.pitch;
-                const float n = (float)at.cnt;
-                if (V > 1 && p.merged == V)
-                    merge<V, V>(to + slot, s1, s2, n);
-                else if (V == 8 && p.merged == 4)
-                    merge<V, 4>(to + slot * 2, s1, s2, n);
-                else if (V > 2 && p.merged == 2)
-                    merge<V, 2>(to + slot * (V / 2), s1, s2, n);
-                else
-                    merge<V, 1>(to + at.j0, s1, s2, n);
             }
         }
         __syncthreads();
@@ -713,8 +827,8 @@ constexpr size_t SMEM = 227 * 1024;
 
 size_t smem_bytes(const GroupNorm &p, int threads, int vec_bytes)
 {
-    return kept_bytes(p, threads, vec_bytes) + (size_t)p.pitch * p.lanes * 8 +
-           (size_t)p.gs * 16;
+    return kept_bytes(p, threads, vec_bytes) + entry_bytes(p) +
+           (size_t)p.fold * threads * sizeof(float2);
 }
 
 // Clusters of `team` blocks that the device holds at once, one block to a
@@ -749,7 +863,7 @@ int clusters_of(const void *fn, int team, int sms)
 template <typename TX, typename TY, int V>
 bool launch(cudaStream_t st, GroupNorm p, int sms)
 {
-    static unsigned done[2] = {0, 0};
+    static unsigned done[4] = {0, 0, 0, 0};
     constexpr int vb = (int)sizeof(TX) * V;
     p.R = 1;
     while (p.R < V && (long)p.R * p.C % V)
@@ -796,7 +910,13 @@ bool launch(cudaStream_t st, GroupNorm p, int sms)
     GroupNorm best = p;
     double best_t = 1e30;
     bool best_grid = false;
-    const void *fn = (const void *)groupnorm_k<TX, TY, V, false>;
+    auto kernel = [&](bool grid, bool folded) {
+        return grid ? (folded ? (const void *)groupnorm_k<TX, TY, V, true, true>
+                              : (const void *)groupnorm_k<TX, TY, V, true, false>)
+                    : (folded ? (const void *)groupnorm_k<TX, TY, V, false, true>
+                              : (const void *)groupnorm_k<TX, TY, V, false, false>);
+    };
+    const void *fn = kernel(false, false);
     if (!tc::smem_opt_in(fn, SMEM, &done[0])) {
         fail("ops_groupnorm_cl: no %zu bytes of shared memory", SMEM);
         return true;
@@ -824,6 +944,7 @@ bool launch(cudaStream_t st, GroupNorm p, int sms)
         const int threads = (q.slots * q.lanes + 31) / 32 * 32;
         const long need = (rows + q.lanes - 1) / q.lanes;
         q.keep = q.ring = 0;
+        q.fold = need > FOLD ? V / q.merged : 0;
         const size_t fixed = smem_bytes(q, threads, vb) + 16;
         if (fixed > SMEM)
             return -1L;
@@ -886,9 +1007,8 @@ bool launch(cudaStream_t st, GroupNorm p, int sms)
         return false;
     const int threads = (best.slots * best.lanes + 31) / 32 * 32;
     const size_t smem = smem_bytes(best, threads, vb);
-    if (best_grid)
-        fn = (const void *)groupnorm_k<TX, TY, V, true>;
-    if (!tc::smem_opt_in(fn, SMEM, &done[best_grid])) {
+    fn = kernel(best_grid, best.fold > 0);
+    if (!tc::smem_opt_in(fn, SMEM, &done[best_grid + 2 * (best.fold > 0)])) {
         fail("ops_groupnorm_cl: no %zu bytes of shared memory", SMEM);
         return true;
     }
