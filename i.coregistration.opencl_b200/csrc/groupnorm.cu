@@ -225,6 +225,16 @@ __device__ __forceinline__ void sums_begin(const GroupNorm &p, const TX *x, cons
     }
 }
 
+// M2 from the sums s1 and s2 about another point, m that point's distance from
+// the mean: not below zero by rounding, but infinite where s2 has passed
+// float's range (the group then has an infinite variance, not one of zero),
+// and NaN where a value is.
+__device__ __forceinline__ float about_mean(float s1, float s2, float m)
+{
+    const float q = s2 - s1 * m;
+    return q >= 0.0f ? q : q < 0.0f ? 0.0f : s2;
+}
+
 // The means and M2 of n values each, in the place of their sums s1 and s2 about x0.
 template <int V, typename F>
 __device__ __forceinline__ void settle(const float x0[V], float s1[V], float s2[V], F inv)
@@ -232,7 +242,7 @@ __device__ __forceinline__ void settle(const float x0[V], float s1[V], float s2[
 #pragma unroll
     for (int e = 0; e < V; e++) {
         const float m = s1[e] * inv(e);
-        s2[e] = fmaxf(s2[e] - s1[e] * m, 0.0f);
+        s2[e] = about_mean(s1[e], s2[e], m);
         s1[e] = x0[e] + m;
     }
 }
@@ -293,14 +303,14 @@ __device__ __forceinline__ void add_up(float &hi, float &lo, float v)
 __device__ __forceinline__ void join(const GroupNorm &p, float2 *entry, float2 *rest, int before,
                                      float m, float q, float w, bool last)
 {
-    float2 hi = make_float2(0.0f, 0.0f), lo = hi;
+    float2 hi = make_float2(m, q), lo = make_float2(0.0f, 0.0f);
     if (before) {
         hi = *entry;
         lo = *rest;
+        const float d = (m - hi.x) - lo.x;
+        add_up(hi.x, lo.x, d * w);
+        add_up(hi.y, lo.y, fmaf(d * d, w * (float)(before * p.merged), q));
     }
-    const float d = (m - hi.x) - lo.x;
-    add_up(hi.x, lo.x, d * w);
-    add_up(hi.y, lo.y, fmaf(d * d, w * (float)(before * p.merged), q));
     if (last)
         hi = make_float2(hi.x + lo.x, hi.y + lo.y);
     else
@@ -663,7 +673,7 @@ groupnorm_k(const __grid_constant__ GroupNorm p)
             q = warp_sum(q);
             if (lane == 0) {
                 const float m = here > 0.0f ? a / here : 0.0f;
-                const float2 s = make_float2(m0 + m, fmaxf(q - a * m, 0.0f));
+                const float2 s = make_float2(m0 + m, about_mean(a, q, m));
                 if (GRID)
                     out[(size_t)g * p.team + rank] = s;
                 else

@@ -205,7 +205,9 @@ size_t ops_groupnorm_cl_bytes(int nimg, long HW, int C, int groups);
  * channels-last maps (HW pixels, at most 2^30, of C channels; image i from X.off + i X.s0 on, pixels X.ld apart):
  * Y = act((x - mean) / sqrt(var + eps) g[c] + b[c]) with the mean and the
  * biased variance of each image's C / groups neighbouring channels over
- * all pixels, held in float32; g and b float32 (both or neither NULL).
+ * all pixels, held in float32; g and b float32 (both or neither NULL). A group
+ * whose squared distances from its mean add up to more than float32 holds (of
+ * values beyond some 1e16) has an infinite variance: Y = act(b).
  * Y may be X (the same offset, strides and type). work: at least
  * ops_groupnorm_cl_bytes() bytes of device memory at a multiple of 16
  * bytes, NULL where that is 0; calls that may overlap in time each need
