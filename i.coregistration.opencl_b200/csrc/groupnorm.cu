@@ -457,17 +457,18 @@ __device__ __forceinline__ void apply(const GroupNorm &p, const TX *x, TY *y, co
     const long sx = p.lanes * (p.R * p.ldx), sy = p.lanes * (p.R * p.ldy);
     int i = at.cnt - 1;
     TY *w = at_row(y, p.ldy, p, at, i);
+    auto act = [&](float v) { return act2<ACT, true>(make_float2(v, 0.0f), p.slope).x; };
     auto one = [&](const Vec<TX, V> &r, TY *to) {
         float f[V];
         if constexpr (V == 1)
-            f[0] = act1<ACT>(fmaf(r.at(0) - mean[0], a[0], b[0]), p.slope);
+            f[0] = act(fmaf(r.at(0) - mean[0], a[0], b[0]));
         else {
 #pragma unroll
             for (int e = 0; e < V; e += 2) {
-                const float2 v = act2<ACT>(make_float2(fmaf(r.at(e) - mean[e], a[e], b[e]),
-                                                       fmaf(r.at(e + 1) - mean[e + 1], a[e + 1],
-                                                            b[e + 1])),
-                                           p.slope);
+                const float2 v = act2<ACT, true>(
+                    make_float2(fmaf(r.at(e) - mean[e], a[e], b[e]),
+                                fmaf(r.at(e + 1) - mean[e + 1], a[e + 1], b[e + 1])),
+                    p.slope);
                 f[e] = v.x;
                 f[e + 1] = v.y;
             }
@@ -515,7 +516,7 @@ __device__ __forceinline__ void apply(const GroupNorm &p, const TX *x, TY *y, co
 #pragma unroll
             for (int e = 0; e < V; e++)
                 if (e < at.tail)
-                    stf(to + e, act1<ACT>(fmaf(ldf(t + e) - mean[e], a[e], b[e]), p.slope));
+                    stf(to + e, act(fmaf(ldf(t + e) - mean[e], a[e], b[e])));
         }
     }
 }

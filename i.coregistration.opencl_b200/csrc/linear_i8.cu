@@ -327,14 +327,6 @@ __device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias)
     return fmaf(__int2float_rn(acc) * sa, sb, bias);
 }
 
-// The activation of a value whose neighbouring column the neighbouring lane has (0
-// behind the last): by the pair, as the tensor-core kernels take it.
-__device__ __forceinline__ float act_beside(float v, int act, float slope)
-{
-    const float other = __shfl_xor_sync(3u << (threadIdx.x % 32 & ~1u), v, 1);
-    return act2_any(make_float2(v, other), act, slope).x;
-}
-
 // Products of depth 0: act(bias) + R.
 template <typename TC>
 __global__ void __launch_bounds__(256)
@@ -344,10 +336,7 @@ i8_empty_k(const I8Gemm g)
     const long n = (long)g.M * g.N;
     for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long)gridDim.x * 256) {
         const long m = e / g.N, c = e - m * g.N, at = m * g.ldc + c;
-        auto value = [&](long j) {
-            return j < g.N ? scaled(0, g.sa[m], g.sb[j], g.bias ? g.bias[j] : 0.0f) : 0.0f;
-        };
-        float v = act2_any(make_float2(value(c), value(c ^ 1)), g.act, g.slope).x;
+        float v = act_any(scaled(0, g.sa[m], g.sb[c], g.bias ? g.bias[c] : 0.0f), g.act, g.slope);
         if (g.R)
             v += ldf((const TC *)g.R + at);
         stf((TC *)g.C + at, v);
@@ -544,13 +533,11 @@ i8_few_k(const I8Gemm g, const Tokens x, int split)
     for (int i = 0; i < 4; i++)
         part[warp][r + 8 * (i / 2)][2 * (lane % 4) + i % 2] = sum[i];
     __syncthreads();
-    for (int m = m0; m < g.M; m += THREADS / channels) {
+    for (int m = m0; out && m < g.M; m += THREADS / channels) {
         int s = 0;
-        for (int i = 0; i < split && out; i++)
+        for (int i = 0; i < split; i++)
             s += part[c / FEW_CH * split + i][c % FEW_CH][m];
-        float v = act_beside(scaled(s, scale[m], sb, bias), g.act, g.slope);
-        if (!out)
-            continue;
+        float v = act_any(scaled(s, scale[m], sb, bias), g.act, g.slope);
         const long at = (long)m * g.ldc + c0 + c;
         if (g.R)
             v += ldf((const TC *)g.R + at);
@@ -638,13 +625,11 @@ i8_dot_k(const I8Gemm g, const Tokens x, int split)
                 part[warp][r][m] = s;
         }
     __syncthreads();
-    for (int m = m0; m < g.M; m += THREADS / channels) {
+    for (int m = m0; out && m < g.M; m += THREADS / channels) {
         int s = 0;
-        for (int i = 0; i < split && out; i++)
+        for (int i = 0; i < split; i++)
             s += part[c / DOT_ROWS * split + i][c % DOT_ROWS][m];
-        float v = act_beside(scaled(s, scale[m], sb, bias), g.act, g.slope);
-        if (!out)
-            continue;
+        float v = act_any(scaled(s, scale[m], sb, bias), g.act, g.slope);
         const long at = (long)m * g.ldc + c0 + c;
         if (g.R)
             v += ldf((const TC *)g.R + at);
