@@ -327,7 +327,8 @@ __device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias)
     return fmaf(__int2float_rn(acc) * sa, sb, bias);
 }
 
-// Products of depth 0: act(bias) + R.
+// Products of depth 0: act(bias) + R. (Nothing wrote the scales of rows without
+// columns: they may hold anything.)
 template <typename TC>
 __global__ void __launch_bounds__(256)
 i8_empty_k(const I8Gemm g)
@@ -336,7 +337,7 @@ i8_empty_k(const I8Gemm g)
     const long n = (long)g.M * g.N;
     for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long)gridDim.x * 256) {
         const long m = e / g.N, c = e - m * g.N, at = m * g.ldc + c;
-        float v = act_any(scaled(0, g.sa[m], g.sb[c], g.bias ? g.bias[c] : 0.0f), g.act, g.slope);
+        float v = act_any(g.bias ? g.bias[c] : 0.0f, g.act, g.slope);
         if (g.R)
             v += ldf((const TC *)g.R + at);
         stf((TC *)g.C + at, v);
@@ -704,20 +705,20 @@ void linear_fused(const struct ocl_backend *ocl, const I8Gemm &g, const View &X,
 void gemm_i8(const struct ocl_backend *ocl, const I8Gemm &g)
 {
     cudaStream_t st = stream_of(ocl);
-    if (streams(g.M, g.N, g.K)) {
-        const Tokens none = {nullptr, 0, 0};
-        if (g.c_bf16)
-            few<__nv_bfloat16, void>(st, g, none, sms_of(ocl));
-        else
-            few<float, void>(st, g, none, sms_of(ocl));
-        return;
-    }
     if (g.K == 0) {
         const unsigned grid = 8 * sms_of(ocl);
         if (g.c_bf16)
             launch_chained(i8_empty_k<__nv_bfloat16>, grid, 256, 0, st, g);
         else
             launch_chained(i8_empty_k<float>, grid, 256, 0, st, g);
+        return;
+    }
+    if (streams(g.M, g.N, g.K)) {
+        const Tokens none = {nullptr, 0, 0};
+        if (g.c_bf16)
+            few<__nv_bfloat16, void>(st, g, none, sms_of(ocl));
+        else
+            few<float, void>(st, g, none, sms_of(ocl));
         return;
     }
     if (!gemm_i8_tc(st, g, sms_of(ocl)))
@@ -870,7 +871,7 @@ static size_t work_scales(int rows) { return ((size_t)rows * 4 + 15) / 16 * 16; 
 
 extern "C" size_t ops_linear_i8_bytes(int rows, int in)
 {
-    return rows <= 0 || in < 0 || fused(rows, in) ? 0 : work_scales(rows) + (size_t)rows * ops_i8_ld(in);
+    return rows <= 0 || in <= 0 || fused(rows, in) ? 0 : work_scales(rows) + (size_t)rows * ops_i8_ld(in);
 }
 
 extern "C" void ops_linear_i8(struct ops *o, int rows, int in, int out, struct opnd X, int xtype,
@@ -906,6 +907,14 @@ extern "C" void ops_linear_i8(struct ops *o, int rows, int in, int out, struct o
         return;
     cudaStream_t st = stream_of(o->ocl);
     Prof p(o->ocl, "linear_i8");
+    if (in == 0) {
+        g.A = nullptr;
+        g.lda = 0;
+        g.sa = nullptr;
+        gemm_i8(o->ocl, g);
+        launch_ok("linear_i8");
+        return;
+    }
     if (!bytes) {
         linear_fused(o->ocl, g, x, xtype);
         launch_ok("linear_i8");

@@ -134,7 +134,8 @@ void ops_quant_i8(struct ops *o, long rows, int C, struct opnd X, int xtype, str
  * bytes and their ld is one too (ops_i8_ld; bytes beyond K are not used).
  * bias is float32 per column or NULL; R is NULL or a buffer of C's type
  * and layout from element roff on, and may be C itself. ctype is the type
- * of C and R. K is at most OPS_I8_MAX_K; K = 0 gives act(bias) + R. Up
+ * of C and R. K is at most OPS_I8_MAX_K; K = 0 gives act(bias) + R,
+ * whatever the scales hold (ops_quant_i8 writes none for rows without columns). Up
  * to 8 rows of small layers run kernels that stream B once, others the
  * tcgen05 integer tensor cores, in deep products of few tiles with the depth
  * split; a row's results are the same bits by all of them. No reference
