@@ -29,6 +29,9 @@ struct GemmArgs {
     int transb;
     void *C;
     long ldc, sc0, sc1;
+    // Columns behind N that are the product's own too, in every row of C, and
+    // may be overwritten (0: what is behind N is left as it is).
+    int cpad;
     int nb, nb1;
     const float *bias;
     int biasrow;

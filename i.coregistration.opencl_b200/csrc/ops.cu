@@ -478,6 +478,7 @@ bool conv2d_tc(struct ops *o, cl_mem in, int C, int H, int W, cl_mem w, cl_mem b
     gg.ldb = kk * Cp;
     gg.transb = 1;
     gg.ldc = ld;
+    gg.cpad = ld - K;
     gg.bias = fptr(b);
     gg.act = act;
     gg.slope = slope;

@@ -927,9 +927,10 @@ struct Ctx {
     int tile;
 };
 
+// cpad: columns behind N that may be overwritten (GemmArgs).
 void gemm_nt(Ctx &c, const char *what, int M, int N, int K, const void *A,
              long lda, DType ta, const void *B, const float *bias, void *C,
-             long ldc, DType tc, int act, bool residual)
+             long ldc, DType tc, int act, bool residual, int cpad = 0)
 {
     GemmArgs g = gemm_args(M, N, K);
     g.A = A;
@@ -939,6 +940,7 @@ void gemm_nt(Ctx &c, const char *what, int M, int N, int K, const void *A,
     g.transb = 1;
     g.C = C;
     g.ldc = ldc;
+    g.cpad = cpad;
     g.bias = bias;
     g.R = residual ? C : nullptr;
     g.act = act;
@@ -1077,7 +1079,7 @@ void vgg2(Ctx &c, int H, int W, int k)
         }
         gemm_nt(c, "vgg2_proj", h * w, I->ref2[r].feat, ref2_in[r], in, ref2_in[r],
                 I->at, I->proj2_w[r], I->proj2_b[r], I->P2[r][k], I->ref2[r].fpitch,
-                I->at, ACTF_NONE, false);
+                I->at, ACTF_NONE, false, I->ref2[r].fpitch - I->ref2[r].feat);
         if (blk < 2) {
             void *out = in == I->v_a ? I->v_b : I->v_a;
             Prof p(c.m->ocl, "maxpool");
@@ -1463,7 +1465,7 @@ void refiner_body(Ctx &c, const Refiner &r, const void *fa, const void *fb,
                 x, r.cinp, at, ACTF_NONE, false);
     }
     gemm_nt(c, "refiner_out", (int)n, r.nout, r.cinp, x, r.cinp, at, r.out_w, r.out_b,
-            I->d_c, DC_PITCH, DT_F32, ACTF_NONE, false);
+            I->d_c, DC_PITCH, DT_F32, ACTF_NONE, false, DC_PITCH - r.nout);
 }
 
 // ConvRefiner s on an hs x ws grid of a pass of size Hf x Wf (scale

@@ -76,7 +76,19 @@ struct TcParams {
     // Epilogue through TMA stores (output tensor map tma_c); else one
     // coalesced store per row.
     int tma_out;
+    // Such stores may pass a row's end (see ends_clean): else the last columns
+    // go out row by row.
+    int clean;
 };
+
+// Whether a TMA store that is clipped at column N of C leaves what is behind it
+// alone: it writes the rest of the row's last 16 bytes too (measured), so the
+// row has to end with them, or they have to be the product's own.
+bool ends_clean(const GemmArgs &g)
+{
+    const long es = g.c == DT_BF16 ? 2 : 4, over = -(g.N * es) & 15;
+    return over <= g.cpad * es;
+}
 
 template <int BN, int STAGES>
 struct Smem {
@@ -370,7 +382,7 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tma_a,
             for (int c0 = cs; c0 < BN && tl.n0 + c0 < p.N; c0 += cstep) {
                 float v[32];
                 tmem_ld32(acc + c0, v);
-                if (p.tma_out) {
+                if (p.tma_out && (p.clean || tl.n0 + c0 + 32 <= p.N)) {
                     // Lane = row: bias, activation and residual on this
                     // row's 32 values, then one TMA store of the warp's 32 x
                     // 32 block (clipped at the matrix or map edges).
@@ -402,7 +414,12 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tma_a,
                     continue;
                 }
                 // Transpose through the staging block (rotated rows: no bank
-                // conflicts either way).
+                // conflicts either way), which a previous store has read.
+                if (p.tma_out) {
+                    if (lane == 0)
+                        bulk_wait_read<0>();
+                    __syncwarp();
+                }
 #pragma unroll
                 for (int j = 0; j < 32; j++)
                     stage[lane * 32 + ((j + lane) & 31)] = v[j];
@@ -706,6 +723,7 @@ bool launch_tc(cudaStream_t st, const GemmArgs &g, int sm_count)
     // least 32 columns, 16-byte aligned rows).
     memset(&mc, 0, sizeof(mc));
     p.tma_out = BN >= 32 && make_map_c(&mc, g.C, g.c == DT_BF16 ? 2 : 4, p, g.ldc);
+    p.clean = ends_clean(g);
     // Persistent: at most one CTA per SM (the shared memory allows one).
     const int grid = (int)(ntiles < sm_count ? ntiles : sm_count);
     if (p.c_bf16) {
@@ -947,8 +965,9 @@ bool gemm_tc(cudaStream_t st, const GemmArgs &g, int sm_count)
         const char *e = getenv("COREG_GEMM256");
         return !(e && e[0] == '0');
     }();
+    const bool clean = tc::ends_clean(g);
     if (t256 && g.amode == 0 && g.act == ACTF_NONE && g.N >= 512 && g.M >= 512 && g.K >= 256 &&
-        ((uintptr_t)g.C & 15) == 0 && (g.ldc * (g.c == DT_BF16 ? 2 : 4)) % 16 == 0) {
+        ((uintptr_t)g.C & 15) == 0 && (g.ldc * (g.c == DT_BF16 ? 2 : 4)) % 16 == 0 && clean) {
         int best = 0;
         double best_u = 0.0;
         for (int bn : {256, 192, 160}) {
@@ -979,9 +998,9 @@ bool gemm_tc(cudaStream_t st, const GemmArgs &g, int sm_count)
             return tc::launch_tc<256, 4>(st, g, sm_count);
     }
     // At most 16 columns: 32-wide tiles where the output takes the TMA-store
-    // epilogue (16-byte aligned rows), else 16-wide ones.
+    // epilogue (16-byte aligned rows and ends), else 16-wide ones.
     const int ces = g.c == DT_BF16 ? 2 : 4;
-    if (g.N <= 16 && (((uintptr_t)g.C & 15) || (g.ldc * ces) % 16))
+    if (g.N <= 16 && (((uintptr_t)g.C & 15) || (g.ldc * ces) % 16 || !clean))
         return tc::launch_tc<16, 8>(st, g, sm_count);
     if (g.N <= 32)
         return tc::launch_tc<32, 8>(st, g, sm_count);
