@@ -1086,6 +1086,27 @@ bool map_view(View *v, const char *fn, const char *what, const struct opnd &m, i
     return true;
 }
 
+// A view of one map as the rows of all: from the first element of the first map
+// to the last of the last, by single rows where the maps lie whole rows apart.
+View all_maps(const View &v, int nimg, long s0)
+{
+    View a = v;
+    if (nimg == 1)
+        return a;
+    if (v.rows == 1) {
+        a.ld = s0; // maps of one pixel: a row each
+        a.rows = nimg;
+    }
+    else if (v.ld > 0 && s0 % v.ld == 0) {
+        a.rows = (nimg - 1) * (s0 / v.ld) + v.rows;
+    }
+    else {
+        a.rows = 1;
+        a.cols = (nimg - 1) * s0 + (v.rows - 1) * v.ld + v.cols;
+    }
+    return a;
+}
+
 }  // namespace
 }  // namespace coreg
 
@@ -1127,9 +1148,10 @@ extern "C" void ops_groupnorm_cl(struct ops *o, int nimg, long HW, int C, int gr
                !view_of(&vb, fn, "beta", b, 0, C, 1, C, 4))))
         return;
     const bool in_place = same_view(x, y) && (nimg == 1 || X.s0 == Y.s0);
-    const long nx = x.span() + (nimg - 1) * X.s0 * x.es, ny = y.span() + (nimg - 1) * Y.s0 * y.es;
-    if ((!in_place && ranges_meet(x.p, nx, y.p, ny)) || (g && (ranges_meet(vg.p, C * 4L, y.p, ny) ||
-                                                              ranges_meet(vb.p, C * 4L, y.p, ny)))) {
+    const View ax = all_maps(x, nimg, X.s0), ay = all_maps(y, nimg, Y.s0);
+    const long nx = ax.span(), ny = ay.span();
+    if ((!in_place && views_meet(ay, ax)) || (g && (ranges_meet(vg.p, C * 4L, y.p, ny) ||
+                                                    ranges_meet(vb.p, C * 4L, y.p, ny)))) {
         fail("%s: the output overlaps an input", fn);
         return;
     }
