@@ -38,7 +38,8 @@ extern "C" void ops_rotary_plan(struct ops_rotary *r, int rot, int axes, int int
     r->rot = rot;
     r->axes = axes;
     r->interleaved = interleaved != 0;
-    r->mscale = scaling == OPS_ROTARY_PARTS ? (float)(0.1 * log(factor) + 1.0) : 1.0f;
+    // (Factors up to 1 slow no frequency down: their logarithm is not positive.)
+    r->mscale = scaling == OPS_ROTARY_PARTS && factor > 1.0 ? (float)(0.1 * log(factor) + 1.0) : 1.0f;
     const long double two_pi = 6.283185307179586476925286766559L;
     long double b = base;
     if (scaling == OPS_ROTARY_NTK && n > 2)

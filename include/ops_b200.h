@@ -182,7 +182,8 @@ struct ops_rotary {
  * (n > 2); PARTS (the "NTK-by-parts" rule of YaRN, Peng et al. 2023)
  * takes g w + (1 - g) w / factor with g = clamp((r - 1) / 31, 0, 1) for r =
  * length w / 2 pi turns over the trained length, and sets mscale to
- * 0.1 ln(factor) + 1 (1 otherwise). Host only; no device is needed. */
+ * 0.1 ln(factor) + 1 for factors above 1 (1 otherwise). Host only; no device
+ * is needed. */
 void ops_rotary_plan(struct ops_rotary *r, int rot, int axes, int interleaved, double base,
                      int scaling, double factor, long length);
 

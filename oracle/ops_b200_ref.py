@@ -70,7 +70,7 @@ def frequencies(rot, axes, base, scaling="none", factor=1.0, length=1):
     if scaling == "parts":
         g = np.clip((length * w / (2 * PI) - 1) / 31, 0, 1)
         w = g * w + (1 - g) * w / factor
-    return w, 0.1 * math.log(factor) + 1 if scaling == "parts" else 1.0
+    return w, 0.1 * math.log(factor) + 1 if scaling == "parts" and factor > 1 else 1.0
 
 
 def rotary(x, pos, nh, d, rot, axes, interleaved, w, m=1.0):
