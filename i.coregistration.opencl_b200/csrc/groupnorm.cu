@@ -880,7 +880,6 @@ bool launch(cudaStream_t st, GroupNorm p, int sms)
     while (p.R < V && (long)p.R * p.C % V)
         p.R *= 2;
     p.nsr = (p.HW + p.R - 1) / p.R;
-    p.wlast = (p.HW - (p.nsr - 1) * p.R) * p.C;
     p.batch = 1;
     p.merged = p.R > 1                       ? 1
                : p.per % V == 0              ? V
@@ -897,9 +896,12 @@ bool launch(cudaStream_t st, GroupNorm p, int sms)
         unit++;
     if (p.R > 1)
         unit = p.groups;
-    const int gmax = (int)((long)MAX_THREADS * V / (p.R * p.per)); // groups whose slots fit a block
+    // Groups whose slots fit a block. (In 64 bits: eight rows of 2^29 + 1 channels
+    // are eight in 32.)
+    const int gmax = (int)((long)MAX_THREADS * V / ((long)p.R * p.per));
     if (unit > gmax && p.groups > gmax)
         return false;
+    p.wlast = (p.HW - (p.nsr - 1) * p.R) * p.C; // (with R > 1 all channels fit a block)
 
     // Every slice width and team size, and grid teams; times in microseconds by
     // a model: memory at 6.5 MB per microsecond over the whole device, at most
@@ -1127,8 +1129,8 @@ extern "C" void ops_groupnorm_cl(struct ops *o, int nimg, long HW, int C, int gr
 
     if (pending() || !type_ok(fn, xtype) || !type_ok(fn, ytype) || !act_ok(fn, act))
         return;
-    if (nimg < 0 || HW < 0 || C < 0 || groups < 1 || C % groups || nimg > 65535 ||
-        HW > 0x40000000L) {
+    if (nimg < 0 || HW < 0 || C < 0 || C > 0x40000000 || groups < 1 || C % groups ||
+        nimg > 65535 || HW > 0x40000000L) {
         fail("%s: %d maps of %ld x %d in %d groups", fn, nimg, HW, C, groups);
         return;
     }

@@ -203,8 +203,9 @@ void ops_rotary(struct ops *o, const struct ops_rotary *r, long rows, int nh, in
 /* Size in bytes of the work buffer of ops_groupnorm_cl (0: none needed). */
 size_t ops_groupnorm_cl_bytes(int nimg, long HW, int C, int groups);
 
-/* Group norm with an activation over nimg (at most 65535)
- * channels-last maps (HW pixels, at most 2^30, of C channels; image i from X.off + i X.s0 on, pixels X.ld apart):
+/* Group norm with an activation over nimg (at most 65535) channels-last maps
+ * (HW pixels of C channels, both at most 2^30; image i from X.off + i X.s0
+ * on, pixels X.ld apart):
  * Y = act((x - mean) / sqrt(var + eps) g[c] + b[c]) with the mean and the
  * biased variance of each image's C / groups neighbouring channels over
  * all pixels, held in float32; g and b float32 (both or neither NULL). A group
