@@ -846,11 +846,10 @@ size_t smem_bytes(const GroupNorm &p, int threads, int vec_bytes)
 // multiprocessor (a team's blocks are those of one GPC: 15 of 8, not 18).
 int clusters_of(const void *fn, int team, int sms)
 {
-    static int known[4] = {0, 0, 0, 0};
-    const int i = team == 1 ? 0 : team == 2 ? 1 : team == 4 ? 2 : 3;
+    static PerDevice known[3];
     if (team == 1)
         return sms;
-    if (!known[i]) {
+    return known[team == 2 ? 0 : team == 4 ? 1 : 2].get([&] {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(sms / team * team);
         cfg.blockDim = dim3(MAX_THREADS);
@@ -866,9 +865,8 @@ int clusters_of(const void *fn, int team, int sms)
             cudaGetLastError();
             n = sms / team > 1 ? sms / team - 1 : 1;
         }
-        known[i] = n;
-    }
-    return known[i];
+        return n;
+    });
 }
 
 template <typename TX, typename TY, int V>

@@ -6,6 +6,8 @@
 
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 #include "ops_b200.h"
 
@@ -129,6 +131,28 @@ inline bool same_view(const View &a, const View &b)
 
 // Multiprocessors of the backend's device.
 inline int sms_of(const struct ocl_backend *ocl) { return ocl->sm_count > 0 ? ocl->sm_count : 148; }
+
+// A number above 0 that a kernel's launches need and each device answers for
+// itself: asked once per device, or, by host threads that call at the same
+// time, more than once.
+constexpr int MAX_DEVICES = 32;
+struct PerDevice {
+    std::atomic<int> known[MAX_DEVICES];
+    template <typename F>
+    int get(F ask)
+    {
+        int dev = -1;
+        cudaGetDevice(&dev);
+        if (dev < 0 || dev >= MAX_DEVICES)
+            return ask();
+        int n = known[dev].load(std::memory_order_relaxed);
+        if (n <= 0) {
+            n = ask();
+            known[dev].store(n, std::memory_order_relaxed);
+        }
+        return n;
+    }
+};
 
 // Launches a kernel whose blocks may start while the stream's previous kernel
 // ends (programmatic stream serialization): every thread of it calls

@@ -907,14 +907,15 @@ bool smem_opt_in(const void *fn, size_t bytes, unsigned *done_mask)
 {
     int dev = 0;
     cudaGetDevice(&dev);
-    if (*done_mask >> (dev & 31) & 1)
+    if (__atomic_load_n(done_mask, __ATOMIC_RELAXED) >> (dev & 31) & 1)
         return true;
     if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) !=
         cudaSuccess) {
         cudaGetLastError();
         return false;
     }
-    *done_mask |= 1u << (dev & 31);
+    // (Host threads may come here at the same time.)
+    __atomic_fetch_or(done_mask, 1u << (dev & 31), __ATOMIC_RELAXED);
     return true;
 }
 

@@ -1028,8 +1028,8 @@ bool launch_split(cudaStream_t st, const I8Gemm &g)
 template <int BN, int ROWS, int S, typename TC>
 int split_clusters()
 {
-    static int known = 0;
-    if (!known) {
+    static PerDevice known;
+    return known.get([] {
         const size_t smem = sizeof(SplitSmem<BN, ROWS>) + 1024;
         const void *fn = (const void *)tc_i8_split_k<BN, ROWS, S, TC>;
         static unsigned done = 0;
@@ -1050,9 +1050,8 @@ int split_clusters()
             cudaGetLastError();
             return 0;
         }
-        known = n;
-    }
-    return known;
+        return n;
+    });
 }
 
 template <typename TC>
