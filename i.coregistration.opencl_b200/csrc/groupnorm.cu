@@ -161,9 +161,11 @@ struct Place {
     int first, cnt, j0, tail;
 };
 
-// First super row of block t of a team.
+// First super row of block t of a team (the end of the last for what is behind it:
+// t * run stays within the map's).
 __device__ __forceinline__ int run_start(const GroupNorm &p, int t)
 {
+    t = min(t, p.team);
     return t * p.run + min(t, p.run_rem);
 }
 
