@@ -680,7 +680,10 @@ bool streams(int M, int N, int K)
 // again, so that it pays for few values only (us in one launch and in two,
 // rows x out x in: 1 x 4096 x 1024 4.7 and 6.7, 8 x 1024 x 512 6.0 and 6.6, 4 x
 // 4096 x 1024 6.2 and 6.8; 8 x 8192 x 1024 11.8 and 7.0, 1 x 4096 x 4096 8.7 and
-// 7.9).
+// 7.9). The rule does not look at the layer's width, as the work buffer's size
+// does not: of wide layers it takes the slower way (1 x 8192 x 512 4.6 and 6.8,
+// 2 x 16384 x 1024 7.8 and 8.3, but 1 x 8192 x 1500 10.6 and 7.5, 4 x 8192 x 1024
+// 10.4 and 7.2, 1 x 65536 x 1024 28.8 and 18.7).
 constexpr int FUSED_VALUES = 4096, FUSED_IN = 2048;
 bool fused(int rows, int in)
 {

@@ -49,8 +49,7 @@ struct View {
 
 // The operand as a view; fails (with the entry point and the operand
 // named) on a NULL buffer, a negative offset, rows that overlap, memory
-// beyond the buffer or a misaligned element. strict: rows must not overlap
-// (ld >= cols); always wanted of outputs.
+// beyond the buffer or a misaligned element.
 inline bool view_of(View *v, const char *fn, const char *what, cl_mem buf, long off, long ld,
                     long rows, long cols, int es)
 {

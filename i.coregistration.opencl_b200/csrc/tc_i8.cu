@@ -499,7 +499,7 @@ tc_i8_k(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUten
 // rows of A, half the rows of B and the sums of its 128 rows; the tensor cores
 // of both read B from both. Per product that is a third less shared memory
 // and L2 traffic than the 128 x 256 tile's, which saves power (these kernels
-// run at the power limit: 25616 x 4096 x 1024 at about 1.3 GHz of 1.9), and
+// run at the power limit: 25616 x 4096 x 1024 at about 1.5 GHz of 1.9), and
 // leaves room for five stages and the columns' scales.
 // The roles are those above, in each CTA; the first of the pair (the leader)
 // alone issues the products, for both:
@@ -955,7 +955,7 @@ bool with_act(int act, F f)
 // Whether 256-wide tiles go to CTA pairs: for deep products (8192 x 8192 x
 // 8192 417 us in pairs, 440 without; 25616 x 1024 x 4096 140 and 148; 3202 x
 // 1024 x 4096 22.8 and 24.1). In shallow ones the epilogue leads, and a pair
-// waits for the slower of its two (25616 x 4096 x 1024 145 and 141).
+// waits for the slower of its two (25616 x 4096 x 1024 139 and 132).
 bool pair_pays(const I8Gemm &g) { return g.M > BM && g.K >= 2048; }
 
 // PAIR: the kernel of CTA pairs (BN 256).

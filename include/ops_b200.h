@@ -135,11 +135,13 @@ void ops_quant_i8(struct ops *o, long rows, int C, struct opnd X, int xtype, str
  * bias is float32 per column or NULL; R is NULL or a buffer of C's type
  * and layout from element roff on, and may be C itself. ctype is the type
  * of C and R. K is at most OPS_I8_MAX_K; K = 0 gives act(bias) + R,
- * whatever the scales hold (ops_quant_i8 writes none for rows without columns). Up
- * to 8 rows of small layers run kernels that stream B once, others the
- * tcgen05 integer tensor cores, in deep products of few tiles with the depth
- * split; a row's results are the same bits by all of them. No reference
- * counterpart (ops_gemm there is float32 only). */
+ * whatever the scales hold (ops_quant_i8 writes none for rows without
+ * columns). A sum times sa is rounded to float32 before sb: it cannot overflow
+ * there for rows of values below 2e31. Up to 8 rows of small layers run
+ * kernels that stream B once, others the tcgen05 integer tensor cores, in deep
+ * products of few tiles with the depth split; a row's results are the same
+ * bits by all of them. No reference counterpart (ops_gemm there is float32
+ * only). */
 void ops_gemm_i8(struct ops *o, int M, int N, int K, struct opnd A, cl_mem sa, struct opnd B,
                  cl_mem sb, cl_mem bias, struct opnd C, int ctype, cl_mem R, long roff, int act,
                  float slope);
