@@ -212,7 +212,8 @@ size_t ops_groupnorm_cl_bytes(int nimg, long HW, int C, int groups);
  * biased variance of each image's C / groups neighbouring channels over
  * all pixels, held in float32; g and b float32 (both or neither NULL). A group
  * whose squared distances from its mean add up to more than float32 holds (of
- * values beyond some 1e16) has an infinite variance: Y = act(b).
+ * values beyond some 1e16) has an infinite variance: Y = act(b); one whose
+ * values themselves add up to more (beyond some 1e30) is NaN.
  * Y may be X (the same offset, strides and type). work: at least
  * ops_groupnorm_cl_bytes() bytes of device memory at a multiple of 16
  * bytes, NULL where that is 0; calls that may overlap in time each need
